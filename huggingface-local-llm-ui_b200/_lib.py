@@ -38,6 +38,26 @@ class ModelConfig(C.Structure):
                 ("no_graph", C.c_int)]
 
 
+class KvConfig(C.Structure):
+    _fields_ = [("n_heads", C.c_int), ("n_kv_heads", C.c_int), ("head_dim", C.c_int), ("kv_type", C.c_int),
+                ("page_tokens", C.c_int), ("n_pages", C.c_int), ("max_pages", C.c_int)]
+
+
+class KvBatch(C.Structure):
+    _fields_ = [("n_seqs", C.c_int), ("n_tokens", C.c_int), ("max_new", C.c_int), ("q_start", C.c_void_p),
+                ("kv_len", C.c_void_p), ("page_table", C.c_void_p)]
+
+
+class Rope(C.Structure):
+    _fields_ = [("rot_dim", C.c_int), ("n_pos", C.c_int), ("cos", C.c_void_p), ("sin", C.c_void_p)]
+
+
+class Prompt(C.Structure):
+    _fields_ = [("n_heads", C.c_int), ("n_kv_heads", C.c_int), ("head_dim", C.c_int), ("type", C.c_int),
+                ("n_seqs", C.c_int), ("n_q", C.c_int), ("n_kv", C.c_int), ("max_new", C.c_int),
+                ("q_start", C.c_void_p), ("kv_start", C.c_void_p)]
+
+
 # (name, restype, argtypes) for every symbol of include/b2q.h
 _VP, _I, _I64, _SZ, _F = C.c_void_p, C.c_int, C.c_int64, C.c_size_t, C.c_float
 _FP = C.POINTER(C.c_float)
@@ -75,6 +95,14 @@ SIGNATURES = [
     ("b2q_sampler_state", C.c_uint64, [C.c_uint64]),
     ("b2q_sample_dev", _I, [_VP, _VP, _I, _F, _F, C.POINTER(C.c_uint64), _U32P, _VP]),
     ("b2q_gdn_step_dev", _I, [_VP, C.POINTER(GdnConfig), _I] + [_VP] * 12),
+    ("b2q_kv_page_bytes", _SZ, [C.POINTER(KvConfig)]),
+    ("b2q_kv_append_dev", _I, [_VP, C.POINTER(KvConfig), C.POINTER(KvBatch), C.POINTER(Rope), _I, _VP, _I64, _VP, _I64,
+                               _VP, _I64, _VP, _VP, _I, _VP]),
+    ("b2q_kv_gather_dev", _I, [_VP, C.POINTER(KvConfig), C.POINTER(KvBatch), _VP, _VP, _VP, _I, _VP]),
+    ("b2q_attn_paged_work_bytes", _SZ, [_VP, C.POINTER(KvConfig), C.POINTER(KvBatch)]),
+    ("b2q_attn_paged_dev", _I, [_VP, C.POINTER(KvConfig), C.POINTER(KvBatch), _VP, _I, _I64, _VP, _F, _VP, _I, _VP,
+                                _SZ, _VP]),
+    ("b2q_attn_prompt_dev", _I, [_VP, C.POINTER(Prompt), _VP, _I64, _VP, _I64, _VP, _I64, _F, _VP, _VP]),
     ("b2q_gguf_open", _I, [C.c_char_p, C.POINTER(_VP)]),
     ("b2q_gguf_close", _I, [_VP]),
     ("b2q_gguf_version", _I, [_VP]),

@@ -13,6 +13,7 @@
 
 #include "../../include/b2q.h"
 #include "internal.h"
+#include "kv_page.cuh"
 
 namespace b2q {
 
@@ -891,8 +892,13 @@ b2q_status b2q_check_device_error(b2q_engine* e) {
   err = cudaMemcpyFromSymbol(&v, g_b2q_device_error, sizeof v);
   if (err == cudaSuccess) err = cudaMemcpyToSymbol(g_b2q_device_error, &zero, sizeof zero);
   if (err != cudaSuccess) return cuda_error(err, "check_device_error: symbol");
+  int bad = 0;
+  if (v == 0) err = cudaMemcpyFromSymbol(&bad, g_b2q_batch_error, sizeof bad);
+  if (err == cudaSuccess && bad) err = cudaMemcpyToSymbol(g_b2q_batch_error, &zero, sizeof zero);
+  if (err != cudaSuccess) return cuda_error(err, "check_device_error: symbol");
   if (v == 3) return set_error(B2Q_ECUDA, "a device-side layout or bounds check failed (b2q_debug_check_site)");
   if (v != 0) return set_error((b2q_status)v, "a device-side bounded wait gave up (code %d)", v);
+  if (bad) return set_error(B2Q_EINVAL, "a position, page or offset of a batch was out of range: its tokens were skipped");
   return B2Q_OK;
 }
 
@@ -913,3 +919,4 @@ b2q_status b2q_debug_check_site(b2q_engine* e, int* site) {
 
 #include "model_api.cuh"
 #include "gguf_api.cuh"
+#include "paged_api.cuh"

@@ -1,0 +1,287 @@
+// paged_api.cuh -- C entry points of the paged 4-bit K/V cache, of the
+// attention over it and of packed prompt attention (included by b2q_api.cu).
+// None of them allocates, synchronises or keeps state: the caller owns the
+// pool, the workspace and the outputs, so calls on different streams do not
+// meet, and every call can be captured into a graph.
+#pragma once
+
+#include "internal.h"
+#include "attn_paged.cuh"
+#include "attn_prompt.cuh"
+
+namespace b2q {
+
+// Makes the engine's device current and the caller's again at the end.
+struct DeviceGuard {
+  int prev = -1;
+  cudaError_t err;
+  explicit DeviceGuard(int dev) {
+    err = cudaGetDevice(&prev);
+    if (err == cudaSuccess && prev != dev) err = cudaSetDevice(dev);
+    else if (err == cudaSuccess) prev = -1;
+  }
+  ~DeviceGuard() {
+    if (prev >= 0) cudaSetDevice(prev);
+  }
+};
+
+static int el_type(int ggml_type) {
+  return ggml_type == B2Q_F32 ? kElF32 : ggml_type == B2Q_F16 ? kElF16 : ggml_type == B2Q_BF16 ? kElBF16 : -1;
+}
+static int el_size(int el) { return el == kElF32 ? 4 : 2; }
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+static b2q_status check_heads(const char* what, int n_heads, int n_kv_heads, int head_dim) {
+  if (n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads || n_heads > 1024)
+    return set_error(B2Q_EINVAL, "%s: %d query heads over %d K/V heads", what, n_heads, n_kv_heads);
+  if (head_dim != 64 && head_dim != 128)
+    return set_error(B2Q_EUNSUP, "%s: head_dim %d (64 and 128 are supported)", what, head_dim);
+  return B2Q_OK;
+}
+
+static b2q_status check_kv_config(const char* what, const b2q_kv_config* c) {
+  if (!c) return set_error(B2Q_EINVAL, "%s: NULL configuration", what);
+  b2q_status s = check_heads(what, c->n_heads, c->n_kv_heads, c->head_dim);
+  if (s != B2Q_OK) return s;
+  if (c->kv_type != B2Q_Q4_0)
+    return set_error(B2Q_EUNSUP, "%s: cache type %d (B2Q_Q4_0 is supported)", what, c->kv_type);
+  if (c->page_tokens < kKvBlk || c->page_tokens % kKvBlk || c->page_tokens > 4096)
+    return set_error(B2Q_EINVAL, "%s: %d tokens a page (a multiple of 16, at most 4096)", what, c->page_tokens);
+  if (c->n_pages <= 0 || c->max_pages <= 0 || (int64_t)c->max_pages * c->page_tokens > (1 << 30))
+    return set_error(B2Q_EINVAL, "%s: bad pool (%d pages, at most %d a sequence)", what, c->n_pages, c->max_pages);
+  return B2Q_OK;
+}
+
+static b2q_status check_kv_batch(const char* what, const b2q_kv_batch* b) {
+  if (!b) return set_error(B2Q_EINVAL, "%s: NULL batch", what);
+  if (b->n_seqs < 0 || b->n_tokens < 0 || b->max_new < 0 || b->n_seqs > 65535)
+    return set_error(B2Q_EINVAL, "%s: bad batch (%d sequences, %d tokens, at most %d new)", what, b->n_seqs, b->n_tokens,
+                     b->max_new);
+  if (!b->q_start || !b->kv_len || !b->page_table) return set_error(B2Q_EINVAL, "%s: NULL array in the batch", what);
+  return B2Q_OK;
+}
+
+// A strided [tokens][heads * D] operand: 16-byte aligned rows that do not overlap.
+static b2q_status check_rows(const char* what, const char* name, const void* p, int64_t stride, int64_t width, int el) {
+  if (!p) return set_error(B2Q_EINVAL, "%s: %s is NULL", what, name);
+  if (!aligned16(p) || (stride * el_size(el)) % 16)
+    return set_error(B2Q_EINVAL, "%s: the rows of %s must start on 16-byte boundaries", what, name);
+  if (stride < width || stride > ((int64_t)1 << 31))
+    return set_error(B2Q_EINVAL, "%s: %s has %lld elements between rows of %lld", what, name, (long long)stride,
+                     (long long)width);
+  return B2Q_OK;
+}
+
+static KvBatch make_batch(const b2q_kv_config& c, const b2q_kv_batch& b) {
+  KvBatch k;
+  k.n_seqs = b.n_seqs;
+  k.n_tokens = b.n_tokens;
+  k.KV = c.n_kv_heads;
+  k.D = c.head_dim;
+  k.page_tokens = c.page_tokens;
+  k.n_pages = c.n_pages;
+  k.max_pages = c.max_pages;
+  k.q_start = b.q_start;
+  k.kv_len = b.kv_len;
+  k.page_table = b.page_table;
+  return k;
+}
+
+// f(integral_constant...) for the element types' and the head width's instances
+template <typename F>
+static void by_type(int el, F f) {
+  if (el == kElF32) f(std::integral_constant<int, kElF32>());
+  else if (el == kElF16) f(std::integral_constant<int, kElF16>());
+  else f(std::integral_constant<int, kElBF16>());
+}
+template <typename F>
+static void by_dim(int D, F f) {
+  if (D == 64) f(std::integral_constant<int, 64>());
+  else f(std::integral_constant<int, 128>());
+}
+
+}  // namespace b2q
+
+extern "C" {
+
+size_t b2q_kv_page_bytes(const b2q_kv_config* cfg) {
+  if (check_kv_config("b2q_kv_page_bytes", cfg) != B2Q_OK) return 0;
+  return (size_t)cfg->n_kv_heads * (cfg->page_tokens / kKvBlk) * kv_blk_bytes(cfg->head_dim);
+}
+
+b2q_status b2q_kv_append_dev(b2q_engine* e, const b2q_kv_config* cfg, const b2q_kv_batch* batch, const b2q_rope* rope,
+                             int x_type, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+                             int64_t v_stride, void* pages, void* q_out, int q_out_type, void* stream) {
+  static const char* const what = "b2q_kv_append_dev";
+  if (!e) return set_error(B2Q_EINVAL, "%s: NULL engine", what);
+  b2q_status s = check_kv_config(what, cfg);
+  if (s == B2Q_OK) s = check_kv_batch(what, batch);
+  if (s != B2Q_OK) return s;
+  if (batch->n_tokens == 0 || batch->n_seqs == 0) return B2Q_OK;  // (empty tensors have NULL addresses)
+  const int xt = el_type(x_type), D = cfg->head_dim;
+  const int ot = q ? el_type(q_out_type) : (int)kElF32;
+  if (xt < 0 || ot < 0) return set_error(B2Q_EUNSUP, "%s: element type %d", what, xt < 0 ? x_type : q_out_type);
+  s = check_rows(what, "k", k, k_stride, (int64_t)cfg->n_kv_heads * D, xt);
+  if (s == B2Q_OK) s = check_rows(what, "v", v, v_stride, (int64_t)cfg->n_kv_heads * D, xt);
+  if (s == B2Q_OK && q) s = check_rows(what, "q", q, q_stride, (int64_t)cfg->n_heads * D, xt);
+  if (s == B2Q_OK && q) s = check_rows(what, "q_out", q_out, (int64_t)cfg->n_heads * D, (int64_t)cfg->n_heads * D, ot);
+  if (s != B2Q_OK) return s;
+  if (!pages || !aligned16(pages)) return set_error(B2Q_EINVAL, "%s: pages must be a 16-byte aligned pointer", what);
+  if (rope && rope->rot_dim) {
+    if (rope->rot_dim < 0 || rope->rot_dim > D || rope->rot_dim % 8 || rope->n_pos <= 0)
+      return set_error(B2Q_EINVAL, "%s: rotation of %d dims (a multiple of 8, at most %d) over %d positions", what,
+                       rope->rot_dim, D, rope->n_pos);
+    if (!rope->cos || !rope->sin || !aligned16(rope->cos) || !aligned16(rope->sin))
+      return set_error(B2Q_EINVAL, "%s: the rotation tables must be 16-byte aligned pointers", what);
+  }
+  DeviceGuard dev(e->device);
+  if (dev.err != cudaSuccess) return cuda_error(dev.err, what);
+  AppendArgs a;
+  a.b = make_batch(*cfg, *batch);
+  a.H = cfg->n_heads;
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.q_stride = q_stride;
+  a.k_stride = k_stride;
+  a.v_stride = v_stride;
+  a.rot_dim = rope ? rope->rot_dim : 0;
+  a.n_pos = rope ? rope->n_pos : 0;
+  a.cos = rope ? rope->cos : nullptr;
+  a.sin = rope ? rope->sin : nullptr;
+  a.pages = static_cast<uint8_t*>(pages);
+  a.q_out = q_out;
+  cudaStream_t st = stream ? (cudaStream_t)stream : e->stream;
+  by_dim(D, [&](auto d) {
+    by_type(xt, [&](auto x) {
+      by_type(ot, [&](auto o) { kv_append_kernel<d(), x(), o()><<<a.b.n_tokens, kAppendThreads, 0, st>>>(a); });
+    });
+  });
+  launch_counted(e, 1);
+  cudaError_t err = cudaGetLastError();
+  return err == cudaSuccess ? B2Q_OK : cuda_error(err, what);
+}
+
+b2q_status b2q_kv_gather_dev(b2q_engine* e, const b2q_kv_config* cfg, const b2q_kv_batch* batch, const void* pages,
+                             void* k_out, void* v_out, int out_type, void* stream) {
+  static const char* const what = "b2q_kv_gather_dev";
+  if (!e) return set_error(B2Q_EINVAL, "%s: NULL engine", what);
+  b2q_status s = check_kv_config(what, cfg);
+  if (s == B2Q_OK) s = check_kv_batch(what, batch);
+  if (s != B2Q_OK) return s;
+  if (batch->n_tokens == 0 || batch->n_seqs == 0) return B2Q_OK;  // (empty tensors have NULL addresses)
+  const int ot = el_type(out_type);
+  if (ot < 0) return set_error(B2Q_EUNSUP, "%s: element type %d", what, out_type);
+  if (!k_out && !v_out) return set_error(B2Q_EINVAL, "%s: neither k_out nor v_out", what);
+  if (!pages || !aligned16(pages) || !aligned16(k_out) || !aligned16(v_out))
+    return set_error(B2Q_EINVAL, "%s: pages, k_out and v_out must be 16-byte aligned", what);
+  DeviceGuard dev(e->device);
+  if (dev.err != cudaSuccess) return cuda_error(dev.err, what);
+  GatherArgs a;
+  a.b = make_batch(*cfg, *batch);
+  a.pages = static_cast<const uint8_t*>(pages);
+  a.k_out = k_out;
+  a.v_out = v_out;
+  cudaStream_t st = stream ? (cudaStream_t)stream : e->stream;
+  by_dim(cfg->head_dim, [&](auto d) {
+    by_type(ot, [&](auto o) { kv_gather_kernel<d(), o()><<<a.b.n_tokens, 256, 0, st>>>(a); });
+  });
+  launch_counted(e, 1);
+  cudaError_t err = cudaGetLastError();
+  return err == cudaSuccess ? B2Q_OK : cuda_error(err, what);
+}
+
+size_t b2q_attn_paged_work_bytes(const b2q_engine* e, const b2q_kv_config* cfg, const b2q_kv_batch* batch) {
+  if (!e || check_kv_config("b2q_attn_paged_work_bytes", cfg) != B2Q_OK ||
+      check_kv_batch("b2q_attn_paged_work_bytes", batch) != B2Q_OK)
+    return 0;
+  return 256;
+}
+
+b2q_status b2q_attn_paged_dev(b2q_engine* e, const b2q_kv_config* cfg, const b2q_kv_batch* batch, const void* q, int q_type,
+                              int64_t q_stride, const void* pages, float scale, void* out, int out_type, void* work,
+                              size_t work_bytes, void* stream) {
+  static const char* const what = "b2q_attn_paged_dev";
+  if (!e) return set_error(B2Q_EINVAL, "%s: NULL engine", what);
+  b2q_status s = check_kv_config(what, cfg);
+  if (s == B2Q_OK) s = check_kv_batch(what, batch);
+  if (s != B2Q_OK) return s;
+  if (batch->n_tokens == 0 || batch->n_seqs == 0) return B2Q_OK;  // (empty tensors have NULL addresses)
+  const int qt = el_type(q_type), ot = el_type(out_type), D = cfg->head_dim;
+  if (qt < 0 || ot < 0) return set_error(B2Q_EUNSUP, "%s: element type %d", what, qt < 0 ? q_type : out_type);
+  s = check_rows(what, "q", q, q_stride, (int64_t)cfg->n_heads * D, qt);
+  if (s == B2Q_OK) s = check_rows(what, "out", out, (int64_t)cfg->n_heads * D, (int64_t)cfg->n_heads * D, ot);
+  if (s != B2Q_OK) return s;
+  if (!pages || !aligned16(pages)) return set_error(B2Q_EINVAL, "%s: pages must be a 16-byte aligned pointer", what);
+  if (!(scale > 0.0f && scale <= 3.0e38f)) return set_error(B2Q_EINVAL, "%s: scale must be positive and finite", what);
+  const size_t need = b2q_attn_paged_work_bytes(e, cfg, batch);
+  if (!work || !aligned16(work) || work_bytes < need)
+    return set_error(B2Q_EINVAL, "%s: a workspace of %zu bytes is needed (%zu given)", what, need, work_bytes);
+  DeviceGuard dev(e->device);
+  if (dev.err != cudaSuccess) return cuda_error(dev.err, what);
+  PagedArgs a;
+  a.b = make_batch(*cfg, *batch);
+  a.H = cfg->n_heads;
+  a.q = q;
+  a.q_stride = q_stride;
+  a.pages = static_cast<const uint8_t*>(pages);
+  a.scale = scale;
+  a.out = out;
+  cudaStream_t st = stream ? (cudaStream_t)stream : e->stream;
+  const unsigned grid = (unsigned)(((int64_t)a.b.n_tokens * a.H + 3) / 4);
+  by_dim(D, [&](auto d) {
+    by_type(qt, [&](auto x) { by_type(ot, [&](auto o) { attn_paged_kernel<d(), x(), o()><<<grid, 128, 0, st>>>(a); }); });
+  });
+  launch_counted(e, 1);
+  cudaError_t err = cudaGetLastError();
+  return err == cudaSuccess ? B2Q_OK : cuda_error(err, what);
+}
+
+b2q_status b2q_attn_prompt_dev(b2q_engine* e, const b2q_prompt* p, const void* q, int64_t q_stride, const void* k,
+                               int64_t k_stride, const void* v, int64_t v_stride, float scale, void* out, void* stream) {
+  static const char* const what = "b2q_attn_prompt_dev";
+  if (!e || !p) return set_error(B2Q_EINVAL, "%s: NULL argument", what);
+  b2q_status s = check_heads(what, p->n_heads, p->n_kv_heads, p->head_dim);
+  if (s != B2Q_OK) return s;
+  const int t = el_type(p->type), D = p->head_dim;
+  if (t != kElF16 && t != kElBF16) return set_error(B2Q_EUNSUP, "%s: element type %d (F16 and BF16 are supported)", what, p->type);
+  if (p->n_seqs < 0 || p->n_q < 0 || p->n_kv < 0 || p->max_new < 0 || p->n_seqs > 65535)
+    return set_error(B2Q_EINVAL, "%s: bad batch (%d sequences, %d queries, %d keys)", what, p->n_seqs, p->n_q, p->n_kv);
+  if (!p->q_start || !p->kv_start) return set_error(B2Q_EINVAL, "%s: NULL offsets", what);
+  if (p->n_q == 0 || p->n_seqs == 0) return B2Q_OK;  // (empty tensors have NULL addresses)
+  s = check_rows(what, "q", q, q_stride, (int64_t)p->n_heads * D, t);
+  if (s == B2Q_OK) s = check_rows(what, "out", out, (int64_t)p->n_heads * D, (int64_t)p->n_heads * D, t);
+  if (s == B2Q_OK && p->n_kv) s = check_rows(what, "k", k, k_stride, (int64_t)p->n_kv_heads * D, t);
+  if (s == B2Q_OK && p->n_kv) s = check_rows(what, "v", v, v_stride, (int64_t)p->n_kv_heads * D, t);
+  if (s != B2Q_OK) return s;
+  if (!(scale > 0.0f && scale <= 3.0e38f)) return set_error(B2Q_EINVAL, "%s: scale must be positive and finite", what);
+  DeviceGuard dev(e->device);
+  if (dev.err != cudaSuccess) return cuda_error(dev.err, what);
+  PromptArgs a;
+  a.H = p->n_heads;
+  a.KV = p->n_kv_heads;
+  a.n_seqs = p->n_seqs;
+  a.n_q = p->n_q;
+  a.n_kv = p->n_kv;
+  a.q_start = p->q_start;
+  a.kv_start = p->kv_start;
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.q_stride = q_stride;
+  a.k_stride = k_stride;
+  a.v_stride = v_stride;
+  a.scale = scale;
+  a.out = out;
+  cudaStream_t st = stream ? (cudaStream_t)stream : e->stream;
+  const unsigned grid = (unsigned)(((int64_t)a.n_q * a.H + 3) / 4);
+  by_dim(D, [&](auto d) {
+    if (t == kElF16) attn_prompt_kernel<d(), kElF16><<<grid, 128, 0, st>>>(a);
+    else attn_prompt_kernel<d(), kElBF16><<<grid, 128, 0, st>>>(a);
+  });
+  launch_counted(e, 1);
+  cudaError_t err = cudaGetLastError();
+  return err == cudaSuccess ? B2Q_OK : cuda_error(err, what);
+}
+
+}  // extern "C"

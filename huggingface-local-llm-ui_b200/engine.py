@@ -180,6 +180,41 @@ class CudaEngine:
     def dequantize_dev(self, raw_ptr: int, dtype: int, n_elems: int, out_ptr: int, stream: int = 0) -> None:
         check(lib().b2q_dequantize_dev(self._h, raw_ptr, dtype, n_elems, out_ptr, stream or None))
 
+    # -- paged K/V cache and attention for many sequences -------------------
+    # `stream` 0 is the engine's own stream, as in the calls above; torch's
+    # legacy default stream is 1 (cudaStreamLegacy).
+    def kv_append_dev(self, cfg, batch, rope, x_type: int, q_ptr: int, q_stride: int, k_ptr: int, k_stride: int,
+                      v_ptr: int, v_stride: int, pages_ptr: int, q_out_ptr: int, q_out_type: int,
+                      stream: int = 0) -> None:
+        """Rotate q and k, write k and v into the pages (rope None: no
+        rotation; q_ptr 0: keys and values only)."""
+        check(lib().b2q_kv_append_dev(self._h, cfg, batch, rope, x_type, q_ptr or None, q_stride, k_ptr, k_stride, v_ptr,
+                                      v_stride, pages_ptr, q_out_ptr or None, q_out_type, stream or None))
+
+    def kv_gather_dev(self, cfg, batch, pages_ptr: int, k_out_ptr: int, v_out_ptr: int, out_type: int,
+                      stream: int = 0) -> None:
+        """Read the batch's rows of the cache back (either output may be 0)."""
+        check(lib().b2q_kv_gather_dev(self._h, cfg, batch, pages_ptr, k_out_ptr or None, v_out_ptr or None, out_type,
+                                      stream or None))
+
+    def attn_paged_work_bytes(self, cfg, batch) -> int:
+        n = int(lib().b2q_attn_paged_work_bytes(self._h, cfg, batch))
+        if n == 0:
+            raise B2QError(1, lib().b2q_last_error().decode())
+        return n
+
+    def attn_paged_dev(self, cfg, batch, q_ptr: int, q_type: int, q_stride: int, pages_ptr: int, scale: float,
+                       out_ptr: int, out_type: int, work_ptr: int, work_bytes: int, stream: int = 0) -> None:
+        """Attention of the batch's tokens over the cache."""
+        check(lib().b2q_attn_paged_dev(self._h, cfg, batch, q_ptr, q_type, q_stride, pages_ptr, scale, out_ptr, out_type,
+                                       work_ptr, work_bytes, stream or None))
+
+    def attn_prompt_dev(self, p, q_ptr: int, q_stride: int, k_ptr: int, k_stride: int, v_ptr: int, v_stride: int,
+                        scale: float, out_ptr: int, stream: int = 0) -> None:
+        """Causal attention over packed prompts."""
+        check(lib().b2q_attn_prompt_dev(self._h, p, q_ptr, q_stride, k_ptr, k_stride, v_ptr, v_stride, scale, out_ptr,
+                                        stream or None))
+
     def time_gemv(self, bufs, x_ptr: int, k: int, reps: int, stream: int = 0, chained: bool = False) -> float:
         """Average device milliseconds of one GEMV launch, rotating `bufs`;
         chained: each launch a programmatic dependent launch of the last."""

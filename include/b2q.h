@@ -307,6 +307,122 @@ b2q_status b2q_gdn_step_dev(b2q_engine* eng, const b2q_gdn_config* cfg, int n_to
                             const float* ssm_a, const float* dt_bias, const float* ssm_norm, float* conv_state,
                             float* ssm_state, float* y, void* stream);
 
+/* ---- Many sequences at once: a paged K/V cache in 4 bits, the attention
+ * over it, and packed prompts ----
+ * For a host that serves several requests with the projections above
+ * (b2q_matmul_group_dev) and keeps the attention state itself.  No
+ * counterpart in the reference, which ran one sequence over an f32 cache
+ * (inference.rs:2423-2424).  All pointers are device pointers; the calls are
+ * asynchronous on `stream` (NULL: the engine's own), allocate nothing, keep
+ * no state between calls and may be captured into a graph; the current
+ * device is left as it was.  Calls on different streams may overlap as long
+ * as none writes what another uses (a workspace belongs to one call at a
+ * time).  Row operands ([tokens][heads * head_dim], `stride` elements from
+ * token to token) start on 16-byte boundaries.  Element types are B2Q_F32,
+ * B2Q_F16 and B2Q_BF16.
+ *
+ * The device arrays of a batch are not trusted: a position, page or offset
+ * out of range is skipped (a row that has no valid place is not written, a
+ * key with no valid page is not attended) and b2q_check_device_error()
+ * returns B2Q_EINVAL once.  A decreasing offset leaves its sequence without
+ * rows. */
+typedef struct {
+  int n_heads;     /* query heads, a multiple of n_kv_heads, at most 1024 */
+  int n_kv_heads;
+  int head_dim;    /* 64 or 128 */
+  int kv_type;     /* B2Q_Q4_0: blocks of 32 values, 4-bit codes and one f16 scale */
+  int page_tokens; /* tokens of a page: a multiple of 16, at most 4096 */
+  int n_pages;     /* pages of the pool */
+  int max_pages;   /* row length of the page table; max_pages * page_tokens <= 2^30 */
+} b2q_kv_config;
+
+/* The tokens of one call.  Sequence s has the packed rows q_start[s] ..
+ * q_start[s+1]-1 (q_start[0] = 0, not decreasing; a sequence may have none);
+ * they are the LAST ones of its kv_len[s] tokens, so row i of n has position
+ * kv_len[s] - n + i.  Position p lies in page page_table[s][p / page_tokens].
+ * Rows from q_start[n_seqs] on are left as they are. */
+typedef struct {
+  int n_seqs;                /* at most 65535 */
+  int n_tokens;              /* rows of q, k, v and the outputs; rows at or past it are not touched */
+  int max_new;               /* most new tokens of a sequence: chooses the tiling, never the result (0: unknown) */
+  const int32_t* q_start;    /* [n_seqs + 1] */
+  const int32_t* kv_len;     /* [n_seqs] */
+  const int32_t* page_table; /* [n_seqs][max_pages] */
+} b2q_kv_batch;
+
+/* Position rotation of the first rot_dim dims (a multiple of 8), pairs
+ * (i, i + rot_dim/2): x' = x cos - y sin, y' = y cos + x sin, with the f32
+ * tables cos / sin [n_pos][rot_dim/2] (16-byte aligned) indexed by position.
+ * A token at or past n_pos is skipped as above. */
+typedef struct {
+  int rot_dim;
+  int n_pos;
+  const float* cos;
+  const float* sin;
+} b2q_rope;
+
+/* Bytes of a page (keys and values of all K/V heads); the pool is
+ * n_pages * this, 16-byte aligned, and needs no initial contents.  0 (and
+ * b2q_last_error) for a bad configuration.  Inside: [n_kv_heads]
+ * [page_tokens / 16] blocks of 16 tokens, 18 * head_dim bytes each: key
+ * codes, key scales [16][head_dim / 32] f16, value codes, value scales; the
+ * order of the codes is described in csrc/kv_page.cuh. */
+size_t b2q_kv_page_bytes(const b2q_kv_config* cfg);
+
+/* Write the batch's keys and values ([n_tokens][n_kv_heads * head_dim],
+ * x_type) into their pages, keys rotated (rope NULL: no rotation).  With q
+ * not NULL the queries [n_tokens][n_heads * head_dim] are rotated into q_out
+ * (contiguous, q_out_type; may be q itself if type and stride are the same).
+ * 32 values: scale = f16(m / -8), m the first value of the largest
+ * magnitude (the scale stays finite), code = clamp(round(x / scale) + 8, 0, 15),
+ * halves to even.  A block with an infinity or NaN reads back as NaN.  Two
+ * rows with the same place in the pool leave either one's or a mixture. */
+b2q_status b2q_kv_append_dev(b2q_engine* eng, const b2q_kv_config* cfg, const b2q_kv_batch* batch, const b2q_rope* rope,
+                             int x_type, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+                             int64_t v_stride, void* pages, void* q_out, int q_out_type, void* stream);
+
+/* Read the batch's rows back: k_out / v_out [n_tokens][n_kv_heads * head_dim]
+ * contiguous, out_type, either may be NULL.  With q_start the running sums
+ * of kv_len this is the whole cache of the sequences, packed for
+ * b2q_attn_prompt_dev. */
+b2q_status b2q_kv_gather_dev(b2q_engine* eng, const b2q_kv_config* cfg, const b2q_kv_batch* batch, const void* pages,
+                             void* k_out, void* v_out, int out_type, void* stream);
+
+/* Attention of the batch's tokens (one or several new ones a sequence, whose
+ * keys and values are appended already) over the cache: query head h reads
+ * K/V head h / (n_heads / n_kv_heads),
+ * out = sum_j p_j v_j / sum_j p_j, p_j = exp(scale * q.k_j), over the
+ * positions j up to the token's own.  A token without keys gives zeros.
+ * Sums and the softmax in f32; f32 queries and the probabilities are carried as
+ * two f16 parts (~2^-22).  out [n_tokens][n_heads * head_dim] contiguous.
+ * `work`: at least b2q_attn_paged_work_bytes() (16-byte aligned; no initial
+ * contents needed). */
+size_t b2q_attn_paged_work_bytes(const b2q_engine* eng, const b2q_kv_config* cfg, const b2q_kv_batch* batch);
+b2q_status b2q_attn_paged_dev(b2q_engine* eng, const b2q_kv_config* cfg, const b2q_kv_batch* batch, const void* q, int q_type,
+                              int64_t q_stride, const void* pages, float scale, void* out, int out_type, void* work,
+                              size_t work_bytes, void* stream);
+
+/* Packed prompts of b2q_attn_prompt_dev: sequence s has the query rows
+ * q_start[s] .. q_start[s+1]-1 and the key rows kv_start[s] ..
+ * kv_start[s+1]-1; its queries are the last ones, so query i of n attends the
+ * keys 0 .. i + l - n of l (l > n: the sequence continues a prefix). */
+typedef struct {
+  int n_heads, n_kv_heads, head_dim; /* as in b2q_kv_config */
+  int type;                          /* B2Q_F16 or B2Q_BF16: q, k, v and out */
+  int n_seqs;                        /* at most 65535 */
+  int n_q, n_kv;                     /* rows of q and out, rows of k and v */
+  int max_new;                       /* most queries of a sequence: chooses the tiling, never the result (0: unknown) */
+  const int32_t* q_start;            /* [n_seqs + 1], device */
+  const int32_t* kv_start;           /* [n_seqs + 1], device */
+} b2q_prompt;
+
+/* Causal attention of packed prompts, query heads grouped as above.  out
+ * [n_q][n_heads * head_dim] contiguous; rows from q_start[n_seqs] on are left
+ * as they are, queries without keys give zeros.  Scores, sums and outputs are
+ * accumulated in f32, the probabilities rounded to `type`. */
+b2q_status b2q_attn_prompt_dev(b2q_engine* eng, const b2q_prompt* p, const void* q, int64_t q_stride, const void* k,
+                               int64_t k_stride, const void* v, int64_t v_stride, float scale, void* out, void* stream);
+
 /* Replaces StandardNativeEngine::clear_state (inference.rs:2688-2693).
  * Also re-arms the persistent decode kernel's barrier counters and all-rank
  * epoch slots (tensor parallelism: every rank calls it, then the ranks meet
@@ -417,7 +533,9 @@ uint64_t b2q_kernel_launch_count(b2q_engine* eng);
 /* Read and clear the device-side error word (B2Q_ETIMEOUT when a bounded
  * wait gave up; B2Q_ECUDA when the persistent decode kernel found its shared
  * memory laid out otherwise than planned, or, in the debug-bounds build, a
- * bounds check failed); synchronises the engine's stream. */
+ * bounds check failed; B2Q_EINVAL when a paged-cache or packed-prompt call
+ * met a position, page or offset out of range); synchronises the engine's
+ * stream, so a caller waits for its own streams first. */
 b2q_status b2q_check_device_error(b2q_engine* eng);
 
 /* Debug-bounds build (libb2q_checks.so, compiled with -DB2Q_CHECKS): 1 when
