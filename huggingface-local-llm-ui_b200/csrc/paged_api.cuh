@@ -100,6 +100,30 @@ static void by_dim(int D, F f) {
   else f(std::integral_constant<int, 128>());
 }
 
+// CTAs of the paged attention: one per SM.
+static int paged_ctas(const b2q_engine* e) { return std::max(1, std::min(e->num_sms, kPgMaxCtas)); }
+static size_t paged_desc_bytes(int ctas) { return ((size_t)ctas * 2 * sizeof(PgDesc) + 255) / 256 * 256; }
+
+template <int D, int NG, bool PSPLIT>
+static cudaError_t launch_paged(const PagedArgs& a, int ctas, cudaStream_t st) {
+  cudaError_t err = cudaFuncSetAttribute(attn_paged_kernel<D, NG, PSPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         pg_smem_bytes(D, NG));
+  if (err != cudaSuccess) return err;
+  attn_paged_kernel<D, NG, PSPLIT><<<ctas, kPgThreads, pg_smem_bytes(D, NG), st>>>(a);
+  err = cudaGetLastError();
+  if (err != cudaSuccess) return err;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(kPgJoinThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, attn_paged_join_kernel<D, NG>, a);
+}
+
 }  // namespace b2q
 
 extern "C" {
@@ -195,7 +219,8 @@ size_t b2q_attn_paged_work_bytes(const b2q_engine* e, const b2q_kv_config* cfg, 
   if (!e || check_kv_config("b2q_attn_paged_work_bytes", cfg) != B2Q_OK ||
       check_kv_batch("b2q_attn_paged_work_bytes", batch) != B2Q_OK)
     return 0;
-  return 256;
+  // descriptors and pieces of the items cut between CTAs (16 rows: either tiling)
+  return paged_desc_bytes(paged_ctas(e)) + (size_t)paged_ctas(e) * 2 * pg_part_floats(cfg->head_dim, 2) * sizeof(float);
 }
 
 b2q_status b2q_attn_paged_dev(b2q_engine* e, const b2q_kv_config* cfg, const b2q_kv_batch* batch, const void* q, int q_type,
@@ -213,6 +238,8 @@ b2q_status b2q_attn_paged_dev(b2q_engine* e, const b2q_kv_config* cfg, const b2q
   if (s == B2Q_OK) s = check_rows(what, "out", out, (int64_t)cfg->n_heads * D, (int64_t)cfg->n_heads * D, ot);
   if (s != B2Q_OK) return s;
   if (!pages || !aligned16(pages)) return set_error(B2Q_EINVAL, "%s: pages must be a 16-byte aligned pointer", what);
+  if ((int64_t)batch->n_tokens * cfg->n_heads > (1 << 30))
+    return set_error(B2Q_EINVAL, "%s: %d tokens of %d heads in one call", what, batch->n_tokens, cfg->n_heads);
   if (!(scale > 0.0f && scale <= 3.0e38f)) return set_error(B2Q_EINVAL, "%s: scale must be positive and finite", what);
   const size_t need = b2q_attn_paged_work_bytes(e, cfg, batch);
   if (!work || !aligned16(work) || work_bytes < need)
@@ -222,18 +249,29 @@ b2q_status b2q_attn_paged_dev(b2q_engine* e, const b2q_kv_config* cfg, const b2q
   PagedArgs a;
   a.b = make_batch(*cfg, *batch);
   a.H = cfg->n_heads;
+  a.G = cfg->n_heads / cfg->n_kv_heads;
   a.q = q;
+  a.q_type = qt;
   a.q_stride = q_stride;
   a.pages = static_cast<const uint8_t*>(pages);
   a.scale = scale;
   a.out = out;
+  a.out_type = ot;
   cudaStream_t st = stream ? (cudaStream_t)stream : e->stream;
-  const unsigned grid = (unsigned)(((int64_t)a.b.n_tokens * a.H + 3) / 4);
+  const int ctas = paged_ctas(e);
+  a.desc = static_cast<PgDesc*>(work);
+  a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(work) + paged_desc_bytes(ctas));
+  // 16 rows to an item where the queries are 16-bit (f32 ones take the matrix
+  // tile's other 8 rows for their second part) and more than 8 rows share a K/V head
+  const bool wide = qt != kElF32 && (int64_t)batch->max_new * a.G > 8;
+  // the probabilities' second part where the output shows it
+  const bool split = ot == kElF32;
+  cudaError_t err = cudaSuccess;
   by_dim(D, [&](auto d) {
-    by_type(qt, [&](auto x) { by_type(ot, [&](auto o) { attn_paged_kernel<d(), x(), o()><<<grid, 128, 0, st>>>(a); }); });
+    if (wide) err = split ? launch_paged<d(), 2, true>(a, ctas, st) : launch_paged<d(), 2, false>(a, ctas, st);
+    else err = split ? launch_paged<d(), 1, true>(a, ctas, st) : launch_paged<d(), 1, false>(a, ctas, st);
   });
-  launch_counted(e, 1);
-  cudaError_t err = cudaGetLastError();
+  launch_counted(e, 2);
   return err == cudaSuccess ? B2Q_OK : cuda_error(err, what);
 }
 

@@ -393,8 +393,9 @@ b2q_status b2q_kv_gather_dev(b2q_engine* eng, const b2q_kv_config* cfg, const b2
  * K/V head h / (n_heads / n_kv_heads),
  * out = sum_j p_j v_j / sum_j p_j, p_j = exp(scale * q.k_j), over the
  * positions j up to the token's own.  A token without keys gives zeros.
- * Sums and the softmax in f32; f32 queries and the probabilities are carried as
- * two f16 parts (~2^-22).  out [n_tokens][n_heads * head_dim] contiguous.
+ * Sums and the softmax in f32; f32 queries are carried as two f16 parts
+ * (~2^-22), and so is a probability times its value's scale where out is f32;
+ * for 16-bit outputs that product is rounded once, to f16.  out [n_tokens][n_heads * head_dim] contiguous.
  * `work`: at least b2q_attn_paged_work_bytes() (16-byte aligned; no initial
  * contents needed). */
 size_t b2q_attn_paged_work_bytes(const b2q_engine* eng, const b2q_kv_config* cfg, const b2q_kv_batch* batch);

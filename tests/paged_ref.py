@@ -129,6 +129,11 @@ class Pool:
             vs.append(values(*kv[1]))
         return ks, vs
 
+    def largest_scale(self):
+        """Of the values' f16 scales."""
+        sc = np.ascontiguousarray(self.pages[..., 17 * self.D:]).view(np.float16).astype(np.float64)
+        return float(np.abs(sc[np.isfinite(sc)]).max(initial=0.0))
+
     def upload(self):
         d = self.dev
         d["q_start"] = torch.from_numpy(self.q_start).cuda()
@@ -144,7 +149,7 @@ class Pool:
                               d["q_start"].data_ptr(), d["kv_len"].data_ptr(), d["table"].data_ptr())
 
 
-def attend(q, ks, vs, news, scale, t_out, e_score, e_prob):
+def attend(q, ks, vs, news, scale, t_out, e_score, e_prob, tiny=0.0):
     """f64 attention of q [T, H, D] (f64) and a bound of each output's error.
 
     With scores off by at most e = e_score * scale * max_j sum_d |q_d k_jd| + 2^-20 (the two
@@ -152,7 +157,8 @@ def attend(q, ks, vs, news, scale, t_out, e_score, e_prob):
     below 8 in magnitude from the maximum's; larger ones weigh less), weights are off by a factor 1 +- 2e and the
     normalised sum by 2 * 2e * sum_j p_j |v_j|; probabilities rounded by e_prob relative add
     e_prob * sum_j p_j |v_j|, f32 sums over l keys with one rounding per 16 keys add
-    (l / 16 + 16) 2^-24 of it, and the output's rounding half_eps(t_out) of the value."""
+    (l / 16 + 16) 2^-24 of it, and the output's rounding half_eps(t_out) of the value.  `tiny` is
+    what a term may lose beside that, whatever its size (below f16's smallest step)."""
     outs, bounds = [], []
     a = 0
     for n, k, v in zip(news, ks, vs):
@@ -177,7 +183,7 @@ def attend(q, ks, vs, news, scale, t_out, e_score, e_prob):
         e = (e_score * mag.masked_fill(hide, 0.0).amax(-1) if l else s.new_zeros(H, n)) + 2.0 ** -20
         e = e.T[..., None]
         outs.append(o)
-        bounds.append((4 * e + e_prob + (l / 16 + 16) * 2.0 ** -24) * wa + half_eps(t_out) * o.abs() + 1e-30)
+        bounds.append((4 * e + e_prob + (l / 16 + 16) * 2.0 ** -24) * wa + half_eps(t_out) * o.abs() + l * tiny + 1e-30)
     if not outs:
         return torch.zeros(0, q.shape[1], q.shape[2], dtype=torch.float64), None
     return torch.cat(outs), torch.cat(bounds)

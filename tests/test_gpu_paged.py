@@ -178,14 +178,30 @@ def run_paged(engine, pool, q, q_type, out_type, scale, max_new=None, work=None,
     return out
 
 
-# the probabilities and f32 queries as two f16 parts: 2^-21 of each product, and
-# f32 sums of them over the head; 16-bit queries enter exactly
-E_SCORE, E_PROB = 2.0 ** -20, 2.0 ** -21
+# f32 queries as two f16 parts: 2^-21 of each product, and f32 sums of them over
+# the head; 16-bit queries enter exactly.  A probability times its scale is two
+# f16 parts where the output is f32 (2^-21), and one, rounded once (2^-11, as
+# f16 half a step), for 16-bit outputs
+E_SCORE = 2.0 ** -20
+
+
+def e_prob(out_type):
+    return 2.0 ** -21 if out_type == F32 else 2.0 ** -11
+
+
+def tiny(pool):
+    """A probability times its scale, the largest possible one at 2^14 or above,
+    is off by at most half of f16's smallest step, 2^-25, as well, so a term by
+    2^-39 of the largest scale times |code - 8| <= 8; the sum of the
+    probabilities is at least 1."""
+    return 2.0 ** -36 * pool.largest_scale()
+
+
 
 
 def check_paged(engine, pool, ks, vs, q, q_type, out_type, scale, **kw):
     out = run_paged(engine, pool, q, q_type, out_type, scale, **kw)
-    want, bound = R.attend(q[:pool.T].double(), ks, vs, pool.news, scale, TYPES[out_type], E_SCORE, E_PROB)
+    want, bound = R.attend(q[:pool.T].double(), ks, vs, pool.news, scale, TYPES[out_type], E_SCORE, e_prob(out_type), tiny(pool))
     R.check_close(out[:pool.T], want, bound)
     assert (out[pool.T:] == 7.0).all()
     engine.check_device_error()
@@ -291,7 +307,7 @@ def test_strided_queries(engine, pkg):
     wide = rand((2, 8 * 64 + 256), 5, F16)
     q = wide[:, :512].reshape(2, 8, 64)
     out = run_paged(engine, pool, wide, F16, F32, 0.125, q_stride=768)
-    want, bound = R.attend(q.double(), ks, vs, pool.news, 0.125, torch.float32, E_SCORE, E_PROB)
+    want, bound = R.attend(q.double(), ks, vs, pool.news, 0.125, torch.float32, E_SCORE, e_prob(F32), tiny(pool))
     R.check_close(out, want, bound)
 
 
