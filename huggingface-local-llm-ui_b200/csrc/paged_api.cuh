@@ -124,6 +124,42 @@ static cudaError_t launch_paged(const PagedArgs& a, int ctas, cudaStream_t st) {
   return cudaLaunchKernelEx(&cfg, attn_paged_join_kernel<D, NG>, a);
 }
 
+// Tensor maps of the prompt attention: boxes with rows of 64 elements (128
+// bytes, 128-byte swizzle).  Queries as (dim, head of the group, K/V head,
+// token), a box of tpt tokens with gp heads each; keys and values as (dim, K/V
+// head, token), a box of 128 tokens.  Rows past the end read as zeros.
+static bool prompt_map(CUtensorMap* m, int type, int rank, const void* p, const cuuint64_t* dims, const cuuint64_t* strides,
+                       const cuuint32_t* box) {
+  const TmapEncodeFn enc = tmap_encoder();
+  const cuuint32_t one[4] = {1u, 1u, 1u, 1u};
+  return enc != nullptr &&
+         enc(m, type == kElF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank,
+             const_cast<void*>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+static bool prompt_map_q(CUtensorMap* m, const PromptArgs& a, int D, int type) {
+  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)a.G, (cuuint64_t)a.KV, (cuuint64_t)a.n_q};
+  const cuuint64_t strides[3] = {(cuuint64_t)D * 2, (cuuint64_t)a.G * D * 2, (cuuint64_t)a.q_stride * 2};
+  const cuuint32_t box[4] = {64u, (cuuint32_t)a.gp, 1u, (cuuint32_t)a.tpt};
+  return prompt_map(m, type, 4, a.q, dims, strides, box);
+}
+static bool prompt_map_kv(CUtensorMap* m, const void* p, int64_t stride, int rows, int KV, int D, int type) {
+  if (rows == 0) return true;  // (no tile is loaded)
+  const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)KV, (cuuint64_t)rows};
+  const cuuint64_t strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)stride * 2};
+  const cuuint32_t box[3] = {64u, 1u, (cuuint32_t)kPrN};
+  return prompt_map(m, type, 3, p, dims, strides, box);
+}
+template <int D, int TYPE>
+static cudaError_t launch_prompt(const PromptArgs& a, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
+                                 unsigned grid, cudaStream_t st) {
+  cudaError_t err = cudaFuncSetAttribute(attn_prompt_kernel<D, TYPE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         pr_smem_bytes(D));
+  if (err != cudaSuccess) return err;
+  attn_prompt_kernel<D, TYPE><<<grid, kPrThreads, pr_smem_bytes(D), st>>>(a, mq, mk, mv);
+  return cudaGetLastError();
+}
+
 }  // namespace b2q
 
 extern "C" {
@@ -311,14 +347,23 @@ b2q_status b2q_attn_prompt_dev(b2q_engine* e, const b2q_prompt* p, const void* q
   a.v_stride = v_stride;
   a.scale = scale;
   a.out = out;
+  a.G = a.H / a.KV;
+  a.gp = std::min(a.G, 64);
+  a.chunks = (a.G + a.gp - 1) / a.gp;
+  a.tpt = kPrM / a.gp;
+  CUtensorMap mq, mk, mv;
+  if (!prompt_map_q(&mq, a, D, t) || !prompt_map_kv(&mk, a.k, a.k_stride, a.n_kv, a.KV, D, t) ||
+      !prompt_map_kv(&mv, a.v, a.v_stride, a.n_kv, a.KV, D, t))
+    return set_error(B2Q_ECUDA, "%s: cuTensorMapEncodeTiled failed", what);
+  const int64_t grid = ((int64_t)(a.n_q / (2 * a.tpt)) + a.n_seqs) * a.KV * a.chunks;
+  if (grid > INT32_MAX) return set_error(B2Q_EINVAL, "%s: %d queries of %d heads in one call", what, a.n_q, a.H);
   cudaStream_t st = stream ? (cudaStream_t)stream : e->stream;
-  const unsigned grid = (unsigned)(((int64_t)a.n_q * a.H + 3) / 4);
+  cudaError_t err = cudaSuccess;
   by_dim(D, [&](auto d) {
-    if (t == kElF16) attn_prompt_kernel<d(), kElF16><<<grid, 128, 0, st>>>(a);
-    else attn_prompt_kernel<d(), kElBF16><<<grid, 128, 0, st>>>(a);
+    err = t == kElF16 ? launch_prompt<d(), kElF16>(a, mq, mk, mv, (unsigned)grid, st)
+                      : launch_prompt<d(), kElBF16>(a, mq, mk, mv, (unsigned)grid, st);
   });
   launch_counted(e, 1);
-  cudaError_t err = cudaGetLastError();
   return err == cudaSuccess ? B2Q_OK : cuda_error(err, what);
 }
 

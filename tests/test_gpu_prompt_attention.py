@@ -35,6 +35,13 @@ def run_prompt(engine, heads, kv, dim, type_, news, lens, q, k, v, scale, max_ne
     return out
 
 
+def tiny(type_, v):
+    """A probability, the largest at 2^7 or above, is off by at most half of f16's
+    smallest step, 2^-25, as well: 2^-32 of the largest value to each key's
+    term, the sum of the probabilities being at least 1.  (bf16 has f32's range.)"""
+    return 2.0 ** -32 * float(v.float().abs().max()) if type_ == F16 and v.numel() else 0.0
+
+
 def check(engine, heads, kv, dim, type_, news, lens, scale=None, spread=1.0, seed=0, extra=0, **kw):
     T, L = sum(news), sum(lens)
     q = rand((T + extra, heads, dim), seed + 1, type_, spread)
@@ -47,7 +54,8 @@ def check(engine, heads, kv, dim, type_, news, lens, scale=None, spread=1.0, see
     rows = [[x[a:b].double().numpy() for a, b in zip(at[:-1], at[1:])] for x in (k, v)]
     # products of 16-bit values in f32 sums: 2^-19 of their magnitudes; the
     # probabilities are rounded to the type, relative to a maximum that may lag
-    want, bound = R.attend(q[:T].double(), rows[0], rows[1], news, scale, TYPES[type_], 2.0 ** -19, R.half_eps(TYPES[type_]))
+    want, bound = R.attend(q[:T].double(), rows[0], rows[1], news, scale, TYPES[type_], 2.0 ** -19, R.half_eps(TYPES[type_]),
+                           tiny(type_, v[:L]))
     if T:
         R.check_close(out[:T], want, bound)
     assert (out[T:] == 7.0).all()  # rows behind the last sequence
@@ -99,7 +107,7 @@ def test_growing_scores(engine, pkg):
         q[:, :, 0] = 16.0
         q, k, v = q.half(), k.half(), rand((L, 1, D), 5, F16)
         out = run_prompt(engine, 2, 1, D, F16, [L], [L], q, k, v, 1.0)
-        want, bound = R.attend(q.double(), [k.double().numpy()], [v.double().numpy()], [L], 1.0, torch.float16, 2.0 ** -19, 2.0 ** -11)
+        want, bound = R.attend(q.double(), [k.double().numpy()], [v.double().numpy()], [L], 1.0, torch.float16, 2.0 ** -19, 2.0 ** -11, tiny(F16, v))
         # scores up to 16 * 131: the exponent's argument is rounded at that size
         R.check_close(out, want, bound + 4 * 2.0 ** -24 * 16 * 131 * 1.45 * 4.0)
 
@@ -129,7 +137,7 @@ def test_values_that_are_not_finite_reach_only_rows_that_see_them(engine, pkg, t
     assert torch.equal(out[330:], ok[330:])
     assert torch.equal(out[:, 2:], ok[:, 2:])  # the other K/V head
     want, bound = R.attend(q[:200].double(), [k[:200].double().numpy()], [v[:200].double().numpy()], [200], 0.1, TYPES[type_],
-                           2.0 ** -19, R.half_eps(TYPES[type_]))
+                           2.0 ** -19, R.half_eps(TYPES[type_]), tiny(type_, v))
     R.check_close(out[:200], want, bound)
     hit = out[200:330, :2, 5].float()
     assert (~torch.isfinite(hit)).all()
@@ -196,3 +204,18 @@ def test_captured_and_replayed_with_other_lengths(engine, pkg):
         torch.cuda.synchronize()
         want = run_prompt(engine, 4, 2, 64, BF16, [mid, end - mid], [mid, end - mid], q, k, v, 0.125)
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("type_", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads,kv,news,lens", [
+    (2, 2, [256, 255, 1], [2300, 2049, 2304]),   # three tiles with the causal edge behind many whole ones
+    (1, 1, [1100], [1100]),
+    (4, 1, [200, 190], [1500, 200]),
+])
+def test_long_prefixes_and_many_tiles(engine, pkg, type_, dim, heads, kv, news, lens):
+    """Key tiles go round the ring several times, and the last tiles wait for
+    the look at their values: again and again the same bits."""
+    out = check(engine, heads, kv, dim, type_, news, lens, extra=130)
+    for _ in range(5):
+        assert torch.equal(out, check(engine, heads, kv, dim, type_, news, lens, extra=130))
