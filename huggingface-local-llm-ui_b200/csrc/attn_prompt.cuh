@@ -188,6 +188,9 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
   uint8_t* qs = base;
   uint8_t* ring = base + 2 * TB;
 
+  pdl_wait();
+  pdl_launch_dependents();
+
   // ---- which rows: blocks of 2 tpt tokens; sequence s owns the slots from
   // q_start[s] / (2 tpt) + s on (increasing in s, and enough for its blocks) ----
   const int bt = 2 * a.tpt, hc = a.KV * a.chunks;

@@ -87,6 +87,22 @@ static KvBatch make_batch(const b2q_kv_config& c, const b2q_kv_batch& b) {
   return k;
 }
 
+// A launch that may start while the one before it on the stream drains; the
+// kernels wait for that one (pdl_wait) before they touch memory.
+static cudaLaunchConfig_t dependent_launch(unsigned grid, unsigned block, size_t smem, cudaStream_t st,
+                                           cudaLaunchAttribute (&attr)[1]) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cfg;
+}
+
 // f(integral_constant...) for the element types' and the head width's instances
 template <typename F>
 static void by_type(int el, F f) {
@@ -109,16 +125,8 @@ static cudaError_t launch_paged(const PagedArgs& a, int ctas, cudaStream_t st) {
   cudaError_t err = cudaFuncSetAttribute(attn_paged_kernel<D, NG, QSPLIT, PSPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          pg_ring_bytes(D, NG));
   if (err != cudaSuccess) return err;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas);
-  cfg.blockDim = dim3(pg_warps(NG) * 32);
-  cfg.dynamicSmemBytes = pg_ring_bytes(D, NG);
-  cfg.stream = st;
   cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cudaLaunchConfig_t cfg = dependent_launch((unsigned)ctas, pg_warps(NG) * 32, pg_ring_bytes(D, NG), st, attr);
   err = cudaLaunchKernelEx(&cfg, attn_paged_kernel<D, NG, QSPLIT, PSPLIT>, a);
   if (err != cudaSuccess) return err;
   cfg.blockDim = dim3(kPgJoinThreads);
@@ -158,8 +166,9 @@ static cudaError_t launch_prompt(const PromptArgs& a, const CUtensorMap& mq, con
   cudaError_t err = cudaFuncSetAttribute(attn_prompt_kernel<D, TYPE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          pr_smem_bytes(D));
   if (err != cudaSuccess) return err;
-  attn_prompt_kernel<D, TYPE><<<grid, kPrThreads, pr_smem_bytes(D), st>>>(a, mq, mk, mv);
-  return cudaGetLastError();
+  cudaLaunchAttribute attr[1];
+  const cudaLaunchConfig_t cfg = dependent_launch(grid, kPrThreads, pr_smem_bytes(D), st, attr);
+  return cudaLaunchKernelEx(&cfg, attn_prompt_kernel<D, TYPE>, a, mq, mk, mv);
 }
 
 }  // namespace b2q
@@ -213,14 +222,21 @@ b2q_status b2q_kv_append_dev(b2q_engine* e, const b2q_kv_config* cfg, const b2q_
   a.sin = rope ? rope->sin : nullptr;
   a.pages = static_cast<uint8_t*>(pages);
   a.q_out = q_out;
-  cudaStream_t st = stream ? (cudaStream_t)stream : e->stream;
+  cudaLaunchAttribute attr[1];
+  // a token to a CTA while that fills the GPU once, then four
+  const int tok = a.b.n_tokens <= 4 * e->num_sms ? 1 : 4;
+  const cudaLaunchConfig_t lc =
+      dependent_launch((unsigned)((a.b.n_tokens + tok - 1) / tok), kAppendThreads, 0, stream ? (cudaStream_t)stream : e->stream, attr);
+  cudaError_t err = cudaSuccess;
   by_dim(D, [&](auto d) {
     by_type(xt, [&](auto x) {
-      by_type(ot, [&](auto o) { kv_append_kernel<d(), x(), o()><<<a.b.n_tokens, kAppendThreads, 0, st>>>(a); });
+      by_type(ot, [&](auto o) {
+        err = tok == 1 ? cudaLaunchKernelEx(&lc, kv_append_kernel<d(), x(), o(), 1>, a)
+                       : cudaLaunchKernelEx(&lc, kv_append_kernel<d(), x(), o(), 4>, a);
+      });
     });
   });
   launch_counted(e, 1);
-  cudaError_t err = cudaGetLastError();
   return err == cudaSuccess ? B2Q_OK : cuda_error(err, what);
 }
 
@@ -244,12 +260,18 @@ b2q_status b2q_kv_gather_dev(b2q_engine* e, const b2q_kv_config* cfg, const b2q_
   a.pages = static_cast<const uint8_t*>(pages);
   a.k_out = k_out;
   a.v_out = v_out;
-  cudaStream_t st = stream ? (cudaStream_t)stream : e->stream;
+  cudaLaunchAttribute attr[1];
+  // heads apart while that brings CTAs to fill the GPU eight times; a CTA keeps two
+  // heads (a turn for each of its warps).  64 rows of 8 heads: 3 us, by whole rows 12.
+  const int gx = (a.b.n_tokens + kGatherRows - 1) / kGatherRows;
+  a.heads = std::max(2, (int)std::min<int64_t>(a.b.KV, ((int64_t)gx * a.b.KV + 8 * e->num_sms - 1) / (8 * e->num_sms)));
+  cudaLaunchConfig_t lc = dependent_launch((unsigned)gx, 256, 0, stream ? (cudaStream_t)stream : e->stream, attr);
+  lc.gridDim.y = (unsigned)((a.b.KV + a.heads - 1) / a.heads);
+  cudaError_t err = cudaSuccess;
   by_dim(cfg->head_dim, [&](auto d) {
-    by_type(ot, [&](auto o) { kv_gather_kernel<d(), o()><<<a.b.n_tokens, 256, 0, st>>>(a); });
+    by_type(ot, [&](auto o) { err = cudaLaunchKernelEx(&lc, kv_gather_kernel<d(), o()>, a); });
   });
   launch_counted(e, 1);
-  cudaError_t err = cudaGetLastError();
   return err == cudaSuccess ? B2Q_OK : cuda_error(err, what);
 }
 
