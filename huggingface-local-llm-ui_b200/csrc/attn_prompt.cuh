@@ -3,17 +3,22 @@
 // and l keys attends the keys j <= i + l - n.
 //
 // S = Q K^T and O += P V run on the 5th-generation tensor cores with their
-// accumulators in TMEM.  A CTA takes two tiles of 128 query rows; a row is a
-// (token, head) pair, the G heads of a K/V head side by side, so that a
-// short prompt fills a tile and each K/V tile is fetched once for all of them.
-// Over the key tiles (128 keys, K and V by TMA into a ring of 32 KB stages at
-// D = 128) the two row tiles take turns: while one's scores go through the
-// softmax the matrix unit works on the other's.
+// accumulators in TMEM.  An item is two tiles of 128 query rows of a K/V head (one
+// where that fills the GPU better); a row is a (token, head) pair, the G heads of a K/V
+// head side by side, so that a short prompt fills a tile and each K/V tile is
+// fetched once for all of them.  Over the key tiles (128 keys, K and V by TMA into
+// a ring of 32 KB stages at D = 128) the two row tiles take turns: while one's
+// scores go through the softmax the matrix unit works on the other's.  One CTA an
+// SM goes from item to item, the next item's loads and first scores under the
+// last one's epilogue.
 //   warps 0-3, 4-7  softmax of row tile 0 / 1: a thread owns a row, reads its
 //                   128 scores out of TMEM, and writes the probabilities over
 //                   them in the 16-bit type, where the P V product reads them;
 //   warp 8          TMA;   warp 9  issues the matrix instructions;
 //   warps 10, 11    look over the value tiles that some row sees only in part.
+// What bounds it: the exponentials.  A 128 x 128 tile is 1024 cycles of ex2 on an SM and
+// 1024 of matrix instructions, so one pair of scores in four takes a polynomial
+// on the FMA units instead, and the rest of the softmax is packed two by two.
 // The running maximum moves only when a row's grows by more than 2^8: until
 // then probabilities up to 2^15 serve as well (they start at 2^7 for the largest,
 // out of f16's subnormals), and the output in TMEM needs no rescaling.  When it
@@ -26,6 +31,7 @@
 
 #include <cuda.h>
 
+#include "attn_paged.cuh"
 #include "gemm_tc.cuh"
 #include "kv_page.cuh"
 
@@ -40,26 +46,15 @@ struct PromptArgs {
   void* out;
   // tiling: heads of a row tile side by side (at most G), chunks of them, tokens of a tile
   int G, gp, chunks, tpt;
+  // items: slots of nq * tpt tokens (nq row tiles) x K/V heads and chunks, late slots first
+  int nq, slots, items;
+  FastDiv d_hc, d_chunks, d_gp, d_bt;
 };
 
 constexpr int kPrThreads = 384, kPrM = 128, kPrN = 128;
 __host__ __device__ constexpr int pr_tile_bytes(int D) { return 128 * D * 2; }  // of queries, keys or values
 __host__ __device__ constexpr int pr_stages(int D) { return D == 128 ? 5 : 8; }
 __host__ __device__ constexpr int pr_smem_bytes(int D) { return (2 + pr_stages(D)) * pr_tile_bytes(D) + 1024; }
-
-// The offsets of one sequence, checked: queries [qa, qe), keys [ka, ke).
-__device__ __forceinline__ bool prompt_seq(const PromptArgs& a, int s, int& qa, int& qe, int& ka, int& ke) {
-  qa = a.q_start[s];
-  qe = a.q_start[s + 1];
-  ka = a.kv_start[s];
-  ke = a.kv_start[s + 1];
-  if (qe == qa) return false;
-  if (qa < 0 || qe < qa || qe > a.n_q || ka < 0 || ke < ka || ke > a.n_kv) {
-    if (qe > qa) kv_batch_error();
-    return false;
-  }
-  return true;
-}
 
 // One row (a token's head) by a warp, one key at a time, from global memory.
 template <int D, typename T>
@@ -166,8 +161,82 @@ __device__ __forceinline__ float pr_exp2(float x) {
   return y;
 }
 
+__device__ __forceinline__ float pr_max3(float a, float b, float c) {  // NaN if one is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 constexpr float kPrLag = 8.0f;    // (log2) growth of a row's maximum that is let pass
 constexpr float kPrShift = 7.0f;  // (log2) the largest probability at a fresh maximum
+
+// Two f32 in a register pair.
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 f2_of(float a, float b) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ f2 f2_of(uint32_t a, uint32_t b) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ void f2_to(f2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f2 f2_fma(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f2 f2_add(f2 a, f2 b) {
+  f2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// 2^x of two numbers at most 2^7 on the FMA units (Cody and Waite's reduction): x =
+// n + f, n whole, |f| <= 1/2, 2^f by a polynomial with the smallest largest relative
+// error on that range (fitted here): degree 3, 7.5e-5, against bf16's half step of
+// 2^-9 of a probability; degree 4, 2.7e-6, against f16's 2^-12.
+template <bool BF>
+__device__ __forceinline__ void pr_exp2_poly(f2 x, float& e0, float& e1) {
+  constexpr float kWhole = 12582912.0f;  // 1.5 * 2^23: a sum with it is rounded to whole numbers
+  float x0, x1;
+  f2_to(x, x0, x1);
+  x = f2_of(fmaxf(x0, -125.0f), fmaxf(x1, -125.0f));  // (below, and masked: 0 at the end)
+  const f2 r = f2_add(x, f2_of(kWhole, kWhole));
+  const f2 f = f2_add(x, f2_fma(r, f2_of(-1.0f, -1.0f), f2_of(kWhole, kWhole)));
+  f2 p;
+  if (BF) {
+    p = f2_fma(f2_of(0.0551716685f, 0.0551716685f), f, f2_of(0.2426111251f, 0.2426111251f));
+    p = f2_fma(p, f, f2_of(0.6932609677f, 0.6932609677f));
+    p = f2_fma(p, f, f2_of(0.9999280572f, 0.9999280572f));
+  } else {
+    p = f2_fma(f2_of(0.0095701022f, 0.0095701022f), f, f2_of(0.0559178591f, 0.0559178591f));
+    p = f2_fma(p, f, f2_of(0.2402474433f, 0.2402474433f));
+    p = f2_fma(p, f, f2_of(0.6931217909f, 0.6931217909f));
+    p = f2_fma(p, f, f2_of(0.9999992847f, 0.9999992847f));
+  }
+  float r0, r1, p0, p1;
+  f2_to(r, r0, r1);
+  f2_to(p, p0, p1);
+  p0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(r0) << 23));
+  p1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(r1) << 23));
+  // less what the smallest x gives, the constant term's 2^-125 of it
+  const float least = -__uint_as_float(__float_as_uint(BF ? 0.9999280572f : 0.9999992847f) - (125u << 23));
+  f2_to(f2_add(f2_of(p0, p1), f2_of(least, least)), e0, e1);
+}
+
+// One item's geometry.
+struct PrItem {
+  int qa, ka, n, l;  // of the sequence: first query and key row, queries, keys
+  int tok0;          // first token of the item within the sequence
+  int nq;            // row tiles with tokens
+  int nt, kt_edge;   // key tiles, the first of them that not every row sees whole
+  int kvh, hoff;     // K/V head, first head of the group
+};
+
+constexpr int kPrSeqs = 192;  // sequences whose offsets are copied to shared memory
 
 template <int D, int TYPE>
 __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid_constant__ PromptArgs a,
@@ -179,52 +248,18 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
   constexpr int NC = D / 64;
   constexpr bool BF = TYPE == kElBF16;
   extern __shared__ uint8_t pr_smem[];
-  __shared__ uint64_t q_full[2], full[NS], empty[NS], v_land[NS], s_full[2], p_full[2], o_full[2], v_ok[NS];
+  __shared__ uint64_t q_full[2], q_empty[2], full[NS], empty[NS], v_land[NS], v_ok[NS], s_full[2], p_full[2], o_full[2], done;
   __shared__ uint32_t s_tmem;
-  __shared__ int s_fail_, s_poison_;
-  volatile int *s_fail = &s_fail_, *s_poison = &s_poison_;
+  __shared__ int s_fail_, s_poison_[8], s_q[kPrSeqs + 1], s_k[kPrSeqs + 1];
+  volatile int *s_fail = &s_fail_, *s_poison = s_poison_;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pr_smem) + 1023) & ~(uintptr_t)1023);
   uint8_t* qs = base;
   uint8_t* ring = base + 2 * TB;
-
-  pdl_wait();
-  pdl_launch_dependents();
-
-  // ---- which rows: blocks of 2 tpt tokens; sequence s owns the slots from
-  // q_start[s] / (2 tpt) + s on (increasing in s, and enough for its blocks) ----
-  const int bt = 2 * a.tpt, hc = a.KV * a.chunks;
-  const int slots = a.n_q / bt + a.n_seqs;
-  const int slot = slots - 1 - (int)(blockIdx.x / hc);  // late blocks, which see the most keys, first
-  const int kvh = (int)(blockIdx.x % hc) / a.chunks, hoff = ((int)(blockIdx.x % hc) % a.chunks) * a.gp;
-  int lo = 0, hi = a.n_seqs - 1;  // the last s with q_start[s] / bt + s <= slot
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (a.q_start[mid] / bt + mid <= slot) lo = mid;
-    else hi = mid - 1;
-  }
-  int qa, qe, ka, ke;
-  if (!prompt_seq(a, lo, qa, qe, ka, ke)) return;
-  const int blk = slot - (qa / bt + lo), n = qe - qa, l = ke - ka;
-  const long long tok0l = (long long)blk * bt;  // first token of the block within the sequence
-  if (blk < 0 || tok0l >= n) return;
-  const int tok0 = (int)tok0l;
-  const int diff = l - n;  // token i attends the keys up to i + diff
-  const int tok_last = min(n, tok0 + bt) - 1;
-  const int kmax = max(0, tok_last + diff + 1);  // keys of the block's last token
-  const int nt = (kmax + kPrN - 1) / kPrN;
-  const int first_lim = tok0 + diff;
-  const int kt_edge = first_lim < 0 ? 0 : (first_lim + 1) / kPrN;  // the first tile that not every row sees whole
-
-  // Value tiles from kt_edge on land on barriers of their own, which the lookers
-  // follow without the uses of the ring before them; their stage's full
-  // barrier is passed at once.  v_land and v_ok are per stage, so that neither can
-  // run a phase ahead of whom it wakes.  Phase of use x: the earlier ones of its stage.
-  auto land_phase = [&](int x) { return (uint32_t)((x - (2 * kt_edge + 1)) / (NS & 1 ? 2 * NS : NS)) & 1u; };
-
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
       mbar_init(&o_full[i], 1);
@@ -235,8 +270,9 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
       mbar_init(&v_land[i], 1);
       mbar_init(&v_ok[i], 2);
     }
+    mbar_init(&done, 1);
     *s_fail = 0;
-    *s_poison = 0;
+    for (int i = 0; i < 8; ++i) s_poison[i] = 0;
     fence_mbar_init();
   }
   if (warp == 9) {
@@ -244,252 +280,379 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  pdl_wait();
+  pdl_launch_dependents();
+  const bool cached = a.n_seqs <= kPrSeqs;
+  if (cached)
+    for (int i = threadIdx.x; i <= a.n_seqs; i += kPrThreads) {
+      s_q[i] = a.q_start[i];
+      s_k[i] = a.kv_start[i];
+    }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s_tmem;  // columns: S0, S1 (128 each), O0, O1
 
-  float sum = 0.0f;  // softmax threads: their row's
+  // ---- items: slots of bt tokens, of which sequence s owns those from
+  // q_start[s] / bt + s on (increasing in s, and enough for it).  CTA b takes b,
+  // then goes back and forth: late slots, which see the most keys, come first,
+  // and what one round gives a CTA too much the next takes from it ----
+  const int bt = a.nq * a.tpt;
+  auto item = [&](int round, PrItem& it) {  // false: nothing to do
+    const int x = round * (int)gridDim.x + ((round & 1) ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x);
+    if (x >= a.items) return false;
+    const int sr = fdiv(x, a.d_hc), hx = x - sr * a.d_hc.d, slot = a.slots - 1 - sr;
+    it.kvh = fdiv(hx, a.d_chunks);
+    it.hoff = (hx - it.kvh * a.chunks) * a.gp;
+    int lo = 0, hi = a.n_seqs - 1;  // the last s with q_start[s] / bt + s <= slot
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      const int qm = cached ? s_q[mid] : a.q_start[mid];
+      if (qm < 0 || fdiv(qm, a.d_bt) + mid <= slot) lo = mid;
+      else hi = mid - 1;
+    }
+    const int qa = cached ? s_q[lo] : a.q_start[lo], qe = cached ? s_q[lo + 1] : a.q_start[lo + 1];
+    const int ka = cached ? s_k[lo] : a.kv_start[lo], ke = cached ? s_k[lo + 1] : a.kv_start[lo + 1];
+    if (qe == qa) return false;
+    if (qa < 0 || qe < qa || qe > a.n_q || ka < 0 || ke < ka || ke > a.n_kv) {
+      if (qe > qa) kv_batch_error();
+      return false;
+    }
+    const int blk = slot - (fdiv(qa, a.d_bt) + lo);
+    const long long tok0 = (long long)blk * bt;
+    if (blk < 0 || tok0 >= qe - qa) return false;
+    it.qa = qa;
+    it.ka = ka;
+    it.n = qe - qa;
+    it.l = ke - ka;
+    it.tok0 = (int)tok0;
+    it.nq = a.nq == 2 && it.tok0 + a.tpt < it.n ? 2 : 1;
+    const int diff = it.l - it.n;  // token i attends the keys up to i + diff
+    const int kmax = max(0, min(it.n, it.tok0 + bt) + diff);
+    it.nt = (kmax + kPrN - 1) / kPrN;
+    const int lim = it.tok0 + diff;
+    it.kt_edge = lim < 0 ? 0 : (lim + 1) / kPrN;
+    return true;
+  };
+  const int rounds = (a.items + (int)gridDim.x - 1) / (int)gridDim.x;
+
   if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     // ---- softmax of row tile i ----
     const int i = warp >> 2, r = threadIdx.x & 127;
-    const int tok = tok0 + i * a.tpt + r / a.gp;
-    const int lim = min(tok + diff, kmax - 1);
-    const int edge = tok0 + i * a.tpt + diff;  // the tile's first token's last key
+    const int tr = fdiv(r, a.d_gp), hr = r - tr * a.gp;  // the row's token and head within the tile
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + lane_base + i * 128, to = tmem + lane_base + 256 + i * D;
     const float c = a.scale * 1.4426950408889634f;
-    float ref = -INFINITY;  // (scores times c)
-    for (int j = 0; j < nt; ++j) {
-      if (!__all_sync(B2Q_FULL, mbar_wait_bounded(&s_full[i], j & 1)) || *s_fail) {
-        *s_fail = 1;
-        break;
+    const f2 c2 = f2_of(c, c);
+    uint32_t s_ph = 0, o_ph = 0;
+    int count = 0;  // items with key tiles, of either row tile
+    bool ok = true;
+    for (int round = 0; ok && round < rounds; ++round) {
+      PrItem it;
+      if (!item(round, it)) continue;
+      if (it.nt > 0) ++count;
+      if (i >= it.nq) continue;
+      const int diff = it.l - it.n, tok = it.tok0 + i * a.tpt + tr, h = it.hoff + hr;
+      const bool live = tr < a.tpt && tok < it.n && h < a.G;
+      const int lim = min(tok + diff, it.l - 1);          // the row's last key
+      const int edge = it.tok0 + i * a.tpt + diff;        // the tile's first token's
+      float ref = -INFINITY, sum = 0.0f;                  // (scores times c)
+      for (int j = 0; j < it.nt; ++j) {
+        ok = __all_sync(B2Q_FULL, mbar_wait_bounded(&s_full[i], s_ph)) && !*s_fail;
+        if (!ok) break;
+        s_ph ^= 1;
+        tc_fence_after();
+        uint32_t s[128];
+        pr_ld32(ts, s);
+        pr_ld32(ts + 32, s + 32);
+        pr_ld32(ts + 64, s + 64);
+        pr_ld32(ts + 96, s + 96);
+        pr_wait_ld();
+        if (j * kPrN + kPrN - 1 > edge) {
+          const int lc = lim - j * kPrN;  // the row's last column
+#pragma unroll
+          for (int x = 0; x < 128; ++x)
+            if (x > lc) s[x] = 0xff800000u;
+        }
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int x = 0; x < 128; x += 8)
+#pragma unroll
+          for (int y = 0; y < 4; ++y)
+            m4[y] = pr_max3(m4[y], __uint_as_float(s[x + 2 * y]), __uint_as_float(s[x + 2 * y + 1]));
+        const float m = pr_max3(pr_max3(m4[0], m4[1], m4[2]), m4[3], m4[3]) * c;
+        if (!(m < INFINITY)) sum = __uint_as_float(0x7fffffffu);  // a score that is NaN or +inf: so is the row
+        const bool move = m > ref + kPrLag;  // (from -inf: any finite maximum)
+        if (__any_sync(B2Q_FULL, move)) {
+          const float al = move ? (ref == -INFINITY ? 0.0f : pr_exp2(ref - m)) : 1.0f;
+          if (move) ref = m;
+          sum *= al;
+          if (j > 0) {
+#pragma unroll 1
+            for (int x = 0; x < D; x += 32) {
+              uint32_t o[32];
+              pr_ld32(to + x, o);
+              pr_wait_ld();
+#pragma unroll
+              for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * al);
+              pr_st32(to + x, o);
+            }
+            pr_wait_st();
+          }
+        }
+        const float off = ref == -INFINITY ? 0.0f : kPrShift - ref;
+        const f2 off2 = f2_of(off, off);
+        f2 t0 = f2_of(0.0f, 0.0f), t1 = t0;
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          uint32_t p[32];
+#pragma unroll
+          for (int x = 0; x < 32; ++x) {
+            const f2 y = f2_fma(f2_of(s[64 * hh + 2 * x], s[64 * hh + 2 * x + 1]), c2, off2);
+            float e0, e1;
+            if ((x & 3) == 3) {
+              pr_exp2_poly<BF>(y, e0, e1);
+            } else {
+              f2_to(y, e0, e1);
+              e0 = pr_exp2(e0);
+              e1 = pr_exp2(e1);
+            }
+            if (x & 1) t1 = f2_add(t1, f2_of(e0, e1));
+            else t0 = f2_add(t0, f2_of(e0, e1));
+            p[x] = el_pack2<T>(e0, e1);
+          }
+          pr_st32(ts + 32 * hh, p);
+        }
+        float u0, u1;
+        f2_to(f2_add(t0, t1), u0, u1);
+        sum += u0 + u1;
+        pr_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[i]);
       }
-      tc_fence_after();
-      uint32_t s[128];
-      pr_ld32(ts, s);
-      pr_ld32(ts + 32, s + 32);
-      pr_ld32(ts + 64, s + 64);
-      pr_ld32(ts + 96, s + 96);
-      pr_wait_ld();
-      if (j * kPrN + kPrN - 1 > edge) {
-        const int lc = lim - j * kPrN;  // the row's last column
-#pragma unroll
-        for (int x = 0; x < 128; ++x)
-          if (x > lc) s[x] = 0xff800000u;
+      if (!ok) break;
+      // ---- epilogue ----
+      if (it.nt > 0) {
+        ok = __all_sync(B2Q_FULL, mbar_wait_bounded(&o_full[i], o_ph)) && !*s_fail;
+        if (!ok) break;
+        o_ph ^= 1;
+        tc_fence_after();
       }
-      float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int x = 0; x < 128; ++x) m4[x & 3] = fmaxf(m4[x & 3], __uint_as_float(s[x]));
-      const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * c;
-      const bool move = m > ref + kPrLag;  // (from -inf: any finite maximum)
-      if (__any_sync(B2Q_FULL, move)) {
-        const float al = move ? (ref == -INFINITY ? 0.0f : pr_exp2(ref - m)) : 1.0f;
-        if (move) ref = m;
-        sum *= al;
-        if (j > 0) {
-#pragma unroll
-          for (int x = 0; x < D; x += 32) {
+      if (it.nt > 0 && s_poison[count & 7] == count) {
+        for (int y = 0; y < 32; ++y) {
+          if (!__shfl_sync(B2Q_FULL, (int)live, y)) continue;
+          const int tk = __shfl_sync(B2Q_FULL, tok, y), hh = __shfl_sync(B2Q_FULL, h, y);
+          prompt_row_slow<D, T>(a, it.qa + tk, it.kvh * a.G + hh, it.ka, tk + diff);
+        }
+      } else {
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        T* orow = reinterpret_cast<T*>(a.out) + ((int64_t)(it.qa + tok) * a.H + it.kvh * a.G + h) * D;
+#pragma unroll 1
+        for (int x = 0; x < D; x += 32) {
+          uint32_t p[16];
+          if (it.nt > 0) {
             uint32_t o[32];
             pr_ld32(to + x, o);
             pr_wait_ld();
 #pragma unroll
-            for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * al);
-            pr_st32(to + x, o);
+            for (int y = 0; y < 16; ++y) p[y] = el_pack2<T>(__uint_as_float(o[2 * y]) * inv, __uint_as_float(o[2 * y + 1]) * inv);
+          } else {
+#pragma unroll
+            for (int y = 0; y < 16; ++y) p[y] = 0u;
           }
-          pr_wait_st();
-        }
-      }
-      const float off = ref == -INFINITY ? 0.0f : kPrShift - ref;
-      float t4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          if (live) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t p[32];
-#pragma unroll
-        for (int x = 0; x < 32; ++x) {
-          const float e0 = pr_exp2(fmaf(__uint_as_float(s[64 * h + 2 * x]), c, off));
-          const float e1 = pr_exp2(fmaf(__uint_as_float(s[64 * h + 2 * x + 1]), c, off));
-          t4[x & 1] += e0;
-          t4[2 + (x & 1)] += e1;
-          p[x] = el_pack2<T>(e0, e1);
+            for (int y = 0; y < 4; ++y)
+              reinterpret_cast<uint4*>(orow + x)[y] = make_uint4(p[4 * y], p[4 * y + 1], p[4 * y + 2], p[4 * y + 3]);
+          }
         }
-        pr_st32(ts + 32 * h, p);
-      }
-      sum += (t4[0] + t4[1]) + (t4[2] + t4[3]);
-      pr_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[i]);
-    }
-  } else if (warp == 8) {
-    // ---- TMA: Q0, K0, Q1, V0, K1, V1, ... ----
-    if (lane == 0) {
-      const uint32_t qbytes = (uint32_t)(a.tpt * a.gp * 128 * NC);
-      int issued = 0;
-      auto load_q = [&](int i) {
-        mbar_arrive_expect_tx(&q_full[i], qbytes);
-        for (int cnk = 0; cnk < NC; ++cnk)
-          tma_load_4d(qs + i * TB + cnk * CB, &mq, cnk * 64, hoff, kvh, qa + tok0 + i * a.tpt, &q_full[i]);
-      };
-      bool ok = true;
-      if (nt > 0) load_q(0);
-      for (int x = 0; x < 2 * nt; ++x) {
-        const int st = x % NS;
-        if (x >= NS && !mbar_wait_bounded(&empty[st], ((x / NS) - 1) & 1)) {
-          ok = false;
-          break;
-        }
-        if (*s_fail) {
-          ok = false;
-          break;
-        }
-        const bool look = (x & 1) && (x >> 1) >= kt_edge;
-        uint64_t* bar = look ? &v_land[st] : &full[st];
-        mbar_arrive_expect_tx(bar, (uint32_t)TB);
-        for (int cnk = 0; cnk < NC; ++cnk)
-          tma_load_3d(ring + st * TB + cnk * CB, (x & 1) ? &mv : &mk, cnk * 64, kvh, ka + (x >> 1) * kPrN, bar);
-        if (look) mbar_arrive(&full[st]);
-        ++issued;
-        if (x == 0) load_q(1);
-      }
-      // copies in flight land before the CTA may end
-      if (!ok) *s_fail = 1;
-      if (nt > 0) mbar_wait_bounded(&q_full[0], 0);
-      if (issued > 0) mbar_wait_bounded(&q_full[1], 0);
-      for (int x = max(0, issued - NS); x < issued; ++x) {
-        if ((x & 1) && (x >> 1) >= kt_edge) mbar_wait_bounded(&v_land[x % NS], land_phase(x));
-        else mbar_wait_bounded(&full[x % NS], (x / NS) & 1);
+        tc_fence_before();  // (the output's reads come before the next item's first product)
       }
     }
-  } else if (warp == 9) {
-    // ---- matrix instructions ----
-    if (lane == 0 && nt > 0) {
-      constexpr uint32_t id_s = pr_idesc(BF, kPrN, false), id_o = pr_idesc(BF, D, true);
-      bool ok = true;
-      auto scores = [&](int i, int st) {  // S_i = Q_i K^T
-        const uint32_t q0 = smem_u32(qs + i * TB), k0 = smem_u32(ring + st * TB);
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t o = (k >> 2) * CB + (k & 3) * 32;
-          pr_mma_ss(tmem + i * 128, pr_desc(q0 + o, 16), pr_desc(k0 + o, 16), id_s, k > 0);
-        }
-        pr_commit(&s_full[i]);
-      };
-      ok = mbar_wait_bounded(&q_full[0], 0) && mbar_wait_bounded(&full[0], 0);
-      if (ok) {
-        tc_fence_after();
-        scores(0, 0);
-        ok = mbar_wait_bounded(&q_full[1], 0);
-        if (ok) {
-          scores(1, 0);
-          pr_commit(&empty[0]);
-        }
-      }
-      for (int j = 0; ok && j < nt; ++j) {
-        const int xv = 2 * j + 1, xk = 2 * j + 2, sv = xv % NS, sk = xk % NS;
-        const bool more = j + 1 < nt;
-        ok = mbar_wait_bounded(&full[sv], (xv / NS) & 1);
-        if (ok && j >= kt_edge) ok = mbar_wait_bounded(&v_ok[sv], land_phase(xv));
-        if (ok && more) ok = mbar_wait_bounded(&full[sk], (xk / NS) & 1);
-        for (int i = 0; ok && i < 2; ++i) {
-          ok = mbar_wait_bounded(&p_full[i], j & 1);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t v0 = smem_u32(ring + sv * TB);
-#pragma unroll
-          for (int k = 0; k < kPrN / 16; ++k)
-            pr_mma_ts(tmem + 256 + i * D, tmem + i * 128 + k * 8, pr_desc(v0 + k * 2048, CB), id_o, j > 0 || k > 0);
-          if (more) scores(i, sk);
-          else pr_commit(&o_full[i]);
-        }
-        if (ok) {
-          pr_commit(&empty[sv]);
-          if (more) pr_commit(&empty[sk]);
-        }
-      }
-      if (!ok) {
-        *s_fail = 1;
-        pr_commit(&o_full[0]);  // (whatever was issued completes before the TMEM is freed)
-        pr_commit(&o_full[1]);
-      }
-    }
+    if (!ok) *s_fail = 1;
   } else {
-    // ---- value tiles that some row sees only in part ----
-    const int w = threadIdx.x - 320;  // 0..63: rows w and w + 64
-    for (int j = kt_edge; j < nt; ++j) {
-      const int x = 2 * j + 1;
-      if (!__all_sync(B2Q_FULL, mbar_wait_bounded(&v_land[x % NS], land_phase(x))) || *s_fail) {
-        *s_fail = 1;
-        break;
-      }
-      uint8_t* vt = ring + (x % NS) * TB;
-      bool bad = false;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int row = w + 64 * h;
-        if (j * kPrN + row >= l) {  // behind the sequence
-          for (int y = 0; y < 8 * NC; ++y)
-            *reinterpret_cast<uint4*>(vt + (y >> 3) * CB + row * 128 + ((y ^ row) & 7) * 16) = make_uint4(0, 0, 0, 0);
-        } else {
-          // an infinity or NaN has all exponent bits set
-          constexpr uint32_t em = BF ? 0x7f80u : 0x7c00u;
-          for (int y = 0; y < 8 * NC; ++y) {
-            const uint4 v = *reinterpret_cast<const uint4*>(vt + (y >> 3) * CB + row * 128 + ((y ^ row) & 7) * 16);
-            const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int z = 0; z < 4; ++z) bad = bad || (u[z] & em) == em || (u[z] & (em << 16)) == (em << 16);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 8) {
+      // ---- TMA: Q0, K0, Q1, V0, K1, V1, ... ----
+      if (lane == 0) {
+        const uint32_t qbytes = (uint32_t)(a.tpt * a.gp * 128 * NC);
+        uint32_t ph = 0, land = 0, q_ph = 0;        // phases: of the ring, bits per stage, bits per row tile
+        uint32_t used = 0, looks = 0;               // for a failure: stages loaded, by which barrier
+        int st = 0, qn = 0;
+        bool ok = true;
+        for (int round = 0; ok && round < rounds; ++round) {
+          PrItem it;
+          if (!item(round, it) || it.nt == 0) continue;
+          auto load_q = [&](int i) {
+            if (!mbar_wait_bounded(&q_empty[i], ((q_ph >> i) & 1) ^ 1)) return false;
+            q_ph ^= 1u << i;
+            qn |= 1 << i;
+            mbar_arrive_expect_tx(&q_full[i], qbytes);
+            for (int cnk = 0; cnk < NC; ++cnk)
+              tma_load_4d(qs + i * TB + cnk * CB, &mq, cnk * 64, it.hoff, it.kvh, it.qa + it.tok0 + i * a.tpt, &q_full[i]);
+            return true;
+          };
+          ok = load_q(0);
+          for (int x = 0; ok && x < 2 * it.nt; ++x) {
+            ok = mbar_wait_bounded(&empty[st], ph ^ 1) && !*s_fail;
+            if (!ok) break;
+            // Value tiles from kt_edge on land on barriers of their own, which the
+            // lookers follow without the uses of the ring before them; their stage's
+            // full barrier is passed at once.  v_land and v_ok are per stage, so that
+            // neither can run a phase ahead of whom it wakes.
+            const bool look = (x & 1) && (x >> 1) >= it.kt_edge;
+            uint64_t* bar = look ? &v_land[st] : &full[st];
+            mbar_arrive_expect_tx(bar, (uint32_t)TB);
+            for (int cnk = 0; cnk < NC; ++cnk)
+              tma_load_3d(ring + st * TB + cnk * CB, (x & 1) ? &mv : &mk, cnk * 64, it.kvh, it.ka + (x >> 1) * kPrN, bar);
+            if (look) {
+              mbar_arrive(&full[st]);
+              land ^= 1u << st;
+            }
+            used |= 1u << st;
+            looks = look ? looks | 1u << st : looks & ~(1u << st);
+            if (++st == NS) {
+              st = 0;
+              ph ^= 1;
+            }
+            if (x == 0 && it.nq == 2) ok = load_q(1);
+          }
+        }
+        if (!ok) {  // copies in flight land before the CTA may end
+          *s_fail = 1;
+          for (int i = 0; i < 2; ++i)
+            if (qn >> i & 1) mbar_wait_bounded(&q_full[i], ((q_ph >> i) & 1) ^ 1);
+          for (int x = 0; x < NS; ++x) {
+            if (!(used >> x & 1)) continue;
+            if (looks >> x & 1) mbar_wait_bounded(&v_land[x], ((land >> x) & 1) ^ 1);
+            else mbar_wait_bounded(&full[x], x < st ? ph : ph ^ 1);
           }
         }
       }
-      if (__any_sync(B2Q_FULL, bad)) *s_poison = 1;
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&v_ok[x % NS]);
-    }
-  }
-
-  __syncwarp();
-
-  // ---- epilogue ----
-  if (warp < 8) {
-    const int i = warp >> 2;
-    if (nt > 0 && !__all_sync(B2Q_FULL, mbar_wait_bounded(&o_full[i], 0))) *s_fail = 1;
-    tc_fence_after();
-  }
-  __syncthreads();
-  if (warp < 8 && !*s_fail) {
-    const int i = warp >> 2, r = threadIdx.x & 127;
-    const int tr = r / a.gp, hg = hoff + r - tr * a.gp, tok = tok0 + i * a.tpt + tr;
-    const bool live = tr < a.tpt && tok < n && hg < a.G;
-    const uint32_t to = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 256 + i * D;
-    if (*s_poison) {
-      for (int y = 0; y < 32; ++y) {
-        if (!__shfl_sync(B2Q_FULL, (int)live, y)) continue;
-        const int tk = __shfl_sync(B2Q_FULL, tok, y), hh = __shfl_sync(B2Q_FULL, hg, y);
-        prompt_row_slow<D, T>(a, qa + tk, kvh * a.G + hh, ka, tk + diff);
+    } else if (warp == 9) {
+      // ---- matrix instructions ----
+      if (lane == 0) {
+        constexpr uint32_t id_s = pr_idesc(BF, kPrN, false), id_o = pr_idesc(BF, D, true);
+        uint32_t ph = 0, land = 0, q_ph = 0, p_ph = 0;
+        int st = 0;
+        bool ok = true;
+        auto next = [&]() {
+          if (++st == NS) {
+            st = 0;
+            ph ^= 1;
+          }
+        };
+        auto scores = [&](int i, int ks) {  // S_i = Q_i K^T
+          const uint32_t q0 = smem_u32(qs + i * TB), k0 = smem_u32(ring + ks * TB);
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t o = (k >> 2) * CB + (k & 3) * 32;
+            pr_mma_ss(tmem + i * 128, pr_desc(q0 + o, 16), pr_desc(k0 + o, 16), id_s, k > 0);
+          }
+          pr_commit(&s_full[i]);
+        };
+        for (int round = 0; ok && round < rounds; ++round) {
+          PrItem it;
+          if (!item(round, it) || it.nt == 0) continue;
+          ok = mbar_wait_bounded(&full[st], ph);
+          for (int i = 0; ok && i < it.nq; ++i) {
+            ok = mbar_wait_bounded(&q_full[i], (q_ph >> i) & 1);
+            if (!ok) break;
+            q_ph ^= 1u << i;
+            tc_fence_after();
+            scores(i, st);
+            if (it.nt == 1) pr_commit(&q_empty[i]);
+          }
+          if (!ok) break;
+          pr_commit(&empty[st]);
+          next();
+          for (int j = 0; ok && j < it.nt; ++j) {
+            const bool more = j + 1 < it.nt;
+            const int sv = st;
+            ok = mbar_wait_bounded(&full[sv], ph);
+            if (ok && j >= it.kt_edge) {
+              ok = mbar_wait_bounded(&v_ok[sv], (land >> sv) & 1);
+              land ^= 1u << sv;
+            }
+            next();
+            const int sk = st;
+            if (ok && more) {
+              ok = mbar_wait_bounded(&full[sk], ph);
+              next();
+            }
+            for (int i = 0; ok && i < it.nq; ++i) {
+              ok = mbar_wait_bounded(&p_full[i], (p_ph >> i) & 1) && !*s_fail;
+              if (!ok) break;
+              p_ph ^= 1u << i;
+              tc_fence_after();
+              const uint32_t v0 = smem_u32(ring + sv * TB);
+#pragma unroll
+              for (int k = 0; k < kPrN / 16; ++k)
+                pr_mma_ts(tmem + 256 + i * D, tmem + i * 128 + k * 8, pr_desc(v0 + k * 2048, CB), id_o, j > 0 || k > 0);
+              if (more) scores(i, sk);
+              else pr_commit(&o_full[i]);
+              if (j + 2 == it.nt) pr_commit(&q_empty[i]);
+            }
+            if (ok) {
+              pr_commit(&empty[sv]);
+              if (more) pr_commit(&empty[sk]);
+            }
+          }
+        }
+        if (!ok) {  // whatever was issued completes before the TMEM is freed
+          *s_fail = 1;
+          pr_commit(&done);
+          mbar_wait_bounded(&done, 0);
+        }
       }
     } else {
-      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-      T* orow = reinterpret_cast<T*>(a.out) + ((int64_t)(qa + tok) * a.H + kvh * a.G + hg) * D;
+      // ---- value tiles that some row sees only in part ----
+      const int w = threadIdx.x - 320;  // 0..63: rows w and w + 64
+      uint32_t land = 0;
+      int x0 = 0, count = 0;  // the item's first stage, items with key tiles
+      bool ok = true;
+      for (int round = 0; ok && round < rounds; ++round) {
+        PrItem it;
+        if (!item(round, it) || it.nt == 0) continue;
+        ++count;
+        for (int j = it.kt_edge; j < it.nt; ++j) {
+          const int st = (x0 + 2 * j + 1) % NS;
+          ok = __all_sync(B2Q_FULL, mbar_wait_bounded(&v_land[st], (land >> st) & 1)) && !*s_fail;
+          if (!ok) break;
+          land ^= 1u << st;
+          uint8_t* vt = ring + st * TB;
+          bool bad = false;
 #pragma unroll
-      for (int x = 0; x < D; x += 32) {
-        uint32_t o[32];
-        if (nt > 0) {
-          pr_ld32(to + x, o);
-          pr_wait_ld();
+          for (int hh = 0; hh < 2; ++hh) {
+            const int row = w + 64 * hh;
+            if (j * kPrN + row >= it.l) {  // behind the sequence
+              for (int y = 0; y < 8 * NC; ++y)
+                *reinterpret_cast<uint4*>(vt + (y >> 3) * CB + row * 128 + ((y ^ row) & 7) * 16) = make_uint4(0, 0, 0, 0);
+            } else {
+              // an infinity or NaN has all exponent bits set
+              constexpr uint32_t em = BF ? 0x7f80u : 0x7c00u;
+#pragma unroll 4
+              for (int y = 0; y < 8 * NC; ++y) {
+                const uint4 v = *reinterpret_cast<const uint4*>(vt + (y >> 3) * CB + row * 128 + ((y ^ row) & 7) * 16);
+                const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int z = 0; z < 4; ++z) bad = bad || (u[z] & em) == em || (u[z] & (em << 16)) == (em << 16);
+              }
+            }
+          }
+          if (__any_sync(B2Q_FULL, bad)) s_poison[count & 7] = count;
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&v_ok[st]);
         }
-        uint32_t p[16];
-#pragma unroll
-        for (int y = 0; y < 16; ++y)
-          p[y] = nt > 0 ? el_pack2<T>(__uint_as_float(o[2 * y]) * inv, __uint_as_float(o[2 * y + 1]) * inv) : 0u;
-        if (live) {
-#pragma unroll
-          for (int y = 0; y < 4; ++y)
-            reinterpret_cast<uint4*>(orow + x)[y] = make_uint4(p[4 * y], p[4 * y + 1], p[4 * y + 2], p[4 * y + 3]);
-        }
+        x0 = (x0 + 2 * it.nt) % NS;
       }
+      if (!ok) *s_fail = 1;
     }
   }
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
   if (warp == 9) {

@@ -393,13 +393,23 @@ b2q_status b2q_attn_prompt_dev(b2q_engine* e, const b2q_prompt* p, const void* q
   if (!prompt_map_q(&mq, a, D, t) || !prompt_map_kv(&mk, a.k, a.k_stride, a.n_kv, a.KV, D, t) ||
       !prompt_map_kv(&mv, a.v, a.v_stride, a.n_kv, a.KV, D, t))
     return set_error(B2Q_ECUDA, "%s: cuTensorMapEncodeTiled failed", what);
-  const int64_t grid = ((int64_t)(a.n_q / (2 * a.tpt)) + a.n_seqs) * a.KV * a.chunks;
-  if (grid > INT32_MAX) return set_error(B2Q_EINVAL, "%s: %d queries of %d heads in one call", what, a.n_q, a.H);
+  // two row tiles to an item, one where that still does not give every SM an item
+  const int64_t hc = (int64_t)a.KV * a.chunks;
+  a.nq = ((int64_t)(a.n_q / a.tpt) + a.n_seqs) * hc <= e->num_sms ? 1 : 2;
+  const int64_t slots = (int64_t)(a.n_q / (a.nq * a.tpt)) + a.n_seqs;
+  if (slots * hc > INT32_MAX - 4096) return set_error(B2Q_EINVAL, "%s: %d queries of %d heads in one call", what, a.n_q, a.H);
+  a.slots = (int)slots;
+  a.items = (int)(slots * hc);
+  a.d_hc = fast_div((int)hc);
+  a.d_chunks = fast_div(a.chunks);
+  a.d_gp = fast_div(a.gp);
+  a.d_bt = fast_div(a.nq * a.tpt);
+  const unsigned grid = (unsigned)std::min<int64_t>(a.items, e->num_sms);
   cudaStream_t st = stream ? (cudaStream_t)stream : e->stream;
   cudaError_t err = cudaSuccess;
   by_dim(D, [&](auto d) {
-    err = t == kElF16 ? launch_prompt<d(), kElF16>(a, mq, mk, mv, (unsigned)grid, st)
-                      : launch_prompt<d(), kElBF16>(a, mq, mk, mv, (unsigned)grid, st);
+    err = t == kElF16 ? launch_prompt<d(), kElF16>(a, mq, mk, mv, grid, st)
+                      : launch_prompt<d(), kElBF16>(a, mq, mk, mv, grid, st);
   });
   launch_counted(e, 1);
   return err == cudaSuccess ? B2Q_OK : cuda_error(err, what);

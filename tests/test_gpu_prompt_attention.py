@@ -42,6 +42,10 @@ def tiny(type_, v):
     return 2.0 ** -32 * float(v.float().abs().max()) if type_ == F16 and v.numel() else 0.0
 
 
+def e_prob(type_):
+    return R.half_eps(TYPES[type_]) + (7.5e-5 if type_ == BF16 else 2.7e-6)
+
+
 def check(engine, heads, kv, dim, type_, news, lens, scale=None, spread=1.0, seed=0, extra=0, **kw):
     T, L = sum(news), sum(lens)
     q = rand((T + extra, heads, dim), seed + 1, type_, spread)
@@ -53,8 +57,9 @@ def check(engine, heads, kv, dim, type_, news, lens, scale=None, spread=1.0, see
     at = np.concatenate([[0], np.cumsum(lens)])
     rows = [[x[a:b].double().numpy() for a, b in zip(at[:-1], at[1:])] for x in (k, v)]
     # products of 16-bit values in f32 sums: 2^-19 of their magnitudes; the
-    # probabilities are rounded to the type, relative to a maximum that may lag
-    want, bound = R.attend(q[:T].double(), rows[0], rows[1], news, scale, TYPES[type_], 2.0 ** -19, R.half_eps(TYPES[type_]),
+    # probabilities are rounded to the type, relative to a maximum that may lag, one
+    # in four after a polynomial that is off by 7.5e-5 (bf16) or 2.7e-6 (f16)
+    want, bound = R.attend(q[:T].double(), rows[0], rows[1], news, scale, TYPES[type_], 2.0 ** -19, e_prob(type_),
                            tiny(type_, v[:L]))
     if T:
         R.check_close(out[:T], want, bound)
@@ -107,7 +112,7 @@ def test_growing_scores(engine, pkg):
         q[:, :, 0] = 16.0
         q, k, v = q.half(), k.half(), rand((L, 1, D), 5, F16)
         out = run_prompt(engine, 2, 1, D, F16, [L], [L], q, k, v, 1.0)
-        want, bound = R.attend(q.double(), [k.double().numpy()], [v.double().numpy()], [L], 1.0, torch.float16, 2.0 ** -19, 2.0 ** -11, tiny(F16, v))
+        want, bound = R.attend(q.double(), [k.double().numpy()], [v.double().numpy()], [L], 1.0, torch.float16, 2.0 ** -19, e_prob(F16), tiny(F16, v))
         # scores up to 16 * 131: the exponent's argument is rounded at that size
         R.check_close(out, want, bound + 4 * 2.0 ** -24 * 16 * 131 * 1.45 * 4.0)
 
@@ -137,7 +142,7 @@ def test_values_that_are_not_finite_reach_only_rows_that_see_them(engine, pkg, t
     assert torch.equal(out[330:], ok[330:])
     assert torch.equal(out[:, 2:], ok[:, 2:])  # the other K/V head
     want, bound = R.attend(q[:200].double(), [k[:200].double().numpy()], [v[:200].double().numpy()], [200], 0.1, TYPES[type_],
-                           2.0 ** -19, R.half_eps(TYPES[type_]), tiny(type_, v))
+                           2.0 ** -19, e_prob(type_), tiny(type_, v))
     R.check_close(out[:200], want, bound)
     hit = out[200:330, :2, 5].float()
     assert (~torch.isfinite(hit)).all()
@@ -156,6 +161,13 @@ def test_keys_and_queries_that_are_not_finite(engine, pkg, bad):
     k2[200, 0, 5] = bad
     out = run_prompt(engine, 4, 2, 128, F16, [330, 60], [330, 60], q, k2, v, 0.1)
     assert torch.equal(out[330:], ok[330:]) and torch.equal(out[:200], ok[:200]) and torch.equal(out[:, 2:], ok[:, 2:])
+    for at in range(200, 216):  # whatever the key's column, the rows whose score is NaN or +inf show it
+        k2 = k.clone()
+        k2[at, 0, 5] = bad
+        got = run_prompt(engine, 4, 2, 128, F16, [330, 60], [330, 60], q, k2, v, 0.1)
+        score = q[at:330, :2, 5].float() * bad
+        hit = torch.isnan(score) | (score == float("inf"))
+        assert torch.equal(torch.isnan(got[at:330, :2].cpu()).all(-1), hit) and torch.isfinite(got[at:330, :2].cpu()[~hit]).all()
     q2 = q.clone()
     q2[150, 1, 3] = float("nan")
     out = run_prompt(engine, 4, 2, 128, F16, [330, 60], [330, 60], q2, k, v, 0.1)
