@@ -16,9 +16,17 @@
 //                   them in the 16-bit type, where the P V product reads them;
 //   warp 8          TMA;   warp 9  issues the matrix instructions;
 //   warps 10, 11    look over the value tiles that some row sees only in part.
-// What bounds it: the exponentials.  A 128 x 128 tile is 1024 cycles of ex2 on an SM and
-// 1024 of matrix instructions, so one pair of scores in four takes a polynomial
-// on the FMA units instead, and the rest of the softmax is packed two by two.
+// What bounds it: the matrix unit (16 instructions of 64 cycles for each row tile
+// and 128 keys, more like 90 with the softmax's TMEM traffic beside them) and, close
+// behind, a softmax of 1640 cycles that has to be done when the other row tile's
+// products are.  Measured at 8192 tokens of 64 heads, 893 us (1.23 PFLOP/s): keeping
+// the issuing warp converged, with one elected thread, 981 -> 910 us (a branch on the
+// lane moved every descriptor between register files); the next item's geometry
+// under the last product and stores of 64 consecutive bytes, 910 -> 893 (16 ragged
+// prompts 172 -> 157).  Tried on the 984 us form: a quarter of the exponentials by a
+// polynomial on the FMA units, 1040; two threads to a row, 1027; key tiles of 64 with two
+// score buffers, 1270 (a score product of 64 keys takes as long as one of
+// 128: its A operand's trip from shared memory).
 // The running maximum moves only when a row's grows by more than 2^8: until
 // then probabilities up to 2^15 serve as well (they start at 2^7 for the largest,
 // out of f16's subnormals), and the output in TMEM needs no rescaling.  When it
@@ -132,6 +140,12 @@ __device__ __forceinline__ void pr_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
 __device__ __forceinline__ void pr_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+// True in one thread of the (converged) warp, the same every time.
+__device__ __forceinline__ bool pr_elect() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
 // 32 columns of the warp's 32 TMEM lanes: a thread's row
 __device__ __forceinline__ void pr_ld32(uint32_t addr, uint32_t* v) {
   asm volatile(
@@ -167,6 +181,16 @@ __device__ __forceinline__ float pr_max3(float a, float b, float c) {  // NaN if
   return r;
 }
 
+// A lane gives `b` (`odd`: `a`) and takes what its partner gives in the place.
+__device__ __forceinline__ void pr_swap(bool odd, int mask, uint4& a, uint4& b) {
+  uint32_t *x = &a.x, *y = &b.x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t got = __shfl_xor_sync(B2Q_FULL, odd ? x[i] : y[i], mask);
+    (odd ? x[i] : y[i]) = got;
+  }
+}
+
 constexpr float kPrLag = 8.0f;    // (log2) growth of a row's maximum that is let pass
 constexpr float kPrShift = 7.0f;  // (log2) the largest probability at a fresh maximum
 
@@ -192,39 +216,6 @@ __device__ __forceinline__ f2 f2_add(f2 a, f2 b) {
   f2 r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
-}
-
-// 2^x of two numbers at most 2^7 on the FMA units (Cody and Waite's reduction): x =
-// n + f, n whole, |f| <= 1/2, 2^f by a polynomial with the smallest largest relative
-// error on that range (fitted here): degree 3, 7.5e-5, against bf16's half step of
-// 2^-9 of a probability; degree 4, 2.7e-6, against f16's 2^-12.
-template <bool BF>
-__device__ __forceinline__ void pr_exp2_poly(f2 x, float& e0, float& e1) {
-  constexpr float kWhole = 12582912.0f;  // 1.5 * 2^23: a sum with it is rounded to whole numbers
-  float x0, x1;
-  f2_to(x, x0, x1);
-  x = f2_of(fmaxf(x0, -125.0f), fmaxf(x1, -125.0f));  // (below, and masked: 0 at the end)
-  const f2 r = f2_add(x, f2_of(kWhole, kWhole));
-  const f2 f = f2_add(x, f2_fma(r, f2_of(-1.0f, -1.0f), f2_of(kWhole, kWhole)));
-  f2 p;
-  if (BF) {
-    p = f2_fma(f2_of(0.0551716685f, 0.0551716685f), f, f2_of(0.2426111251f, 0.2426111251f));
-    p = f2_fma(p, f, f2_of(0.6932609677f, 0.6932609677f));
-    p = f2_fma(p, f, f2_of(0.9999280572f, 0.9999280572f));
-  } else {
-    p = f2_fma(f2_of(0.0095701022f, 0.0095701022f), f, f2_of(0.0559178591f, 0.0559178591f));
-    p = f2_fma(p, f, f2_of(0.2402474433f, 0.2402474433f));
-    p = f2_fma(p, f, f2_of(0.6931217909f, 0.6931217909f));
-    p = f2_fma(p, f, f2_of(0.9999992847f, 0.9999992847f));
-  }
-  float r0, r1, p0, p1;
-  f2_to(r, r0, r1);
-  f2_to(p, p0, p1);
-  p0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(r0) << 23));
-  p1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(r1) << 23));
-  // less what the smallest x gives, the constant term's 2^-125 of it
-  const float least = -__uint_as_float(__float_as_uint(BF ? 0.9999280572f : 0.9999992847f) - (125u << 23));
-  f2_to(f2_add(f2_of(p0, p1), f2_of(least, least)), e0, e1);
 }
 
 // One item's geometry.
@@ -348,11 +339,19 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
     uint32_t s_ph = 0, o_ph = 0;
     int count = 0;  // items with key tiles, of either row tile
     bool ok = true;
-    for (int round = 0; ok && round < rounds; ++round) {
-      PrItem it;
-      if (!item(round, it)) continue;
-      if (it.nt > 0) ++count;
-      if (i >= it.nq) continue;
+    int round = -1;
+    auto next_item = [&](PrItem& it) {  // the next item with this row tile
+      while (++round < rounds) {
+        if (!item(round, it)) continue;
+        if (it.nt > 0) ++count;
+        if (i < it.nq) return true;
+      }
+      return false;
+    };
+    PrItem it;
+    bool more = next_item(it);
+    while (ok && more) {
+      const int mine = count;  // (the item's)
       const int diff = it.l - it.n, tok = it.tok0 + i * a.tpt + tr, h = it.hoff + hr;
       const bool live = tr < a.tpt && tok < it.n && h < a.G;
       const int lim = min(tok + diff, it.l - 1);          // the row's last key
@@ -411,13 +410,9 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
           for (int x = 0; x < 32; ++x) {
             const f2 y = f2_fma(f2_of(s[64 * hh + 2 * x], s[64 * hh + 2 * x + 1]), c2, off2);
             float e0, e1;
-            if ((x & 3) == 3) {
-              pr_exp2_poly<BF>(y, e0, e1);
-            } else {
-              f2_to(y, e0, e1);
-              e0 = pr_exp2(e0);
-              e1 = pr_exp2(e1);
-            }
+            f2_to(y, e0, e1);
+            e0 = pr_exp2(e0);
+            e1 = pr_exp2(e1);
             if (x & 1) t1 = f2_add(t1, f2_of(e0, e1));
             else t0 = f2_add(t0, f2_of(e0, e1));
             p[x] = el_pack2<T>(e0, e1);
@@ -433,14 +428,16 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
         if (lane == 0) mbar_arrive(&p_full[i]);
       }
       if (!ok) break;
-      // ---- epilogue ----
+      // ---- epilogue: the next item's geometry under the last product ----
+      PrItem nx;
+      more = next_item(nx);
       if (it.nt > 0) {
         ok = __all_sync(B2Q_FULL, mbar_wait_bounded(&o_full[i], o_ph)) && !*s_fail;
         if (!ok) break;
         o_ph ^= 1;
         tc_fence_after();
       }
-      if (it.nt > 0 && s_poison[count & 7] == count) {
+      if (it.nt > 0 && s_poison[mine & 7] == mine) {
         for (int y = 0; y < 32; ++y) {
           if (!__shfl_sync(B2Q_FULL, (int)live, y)) continue;
           const int tk = __shfl_sync(B2Q_FULL, tok, y), hh = __shfl_sync(B2Q_FULL, h, y);
@@ -448,28 +445,43 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
         }
       } else {
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        T* orow = reinterpret_cast<T*>(a.out) + ((int64_t)(it.qa + tok) * a.H + it.kvh * a.G + h) * D;
+        // four lanes exchange 16-byte pieces, so that each store writes 64
+        // consecutive bytes of a row: lane y of the four piece y of all four rows
+        const long long at = live ? ((long long)(it.qa + tok) * a.H + it.kvh * a.G + h) * D : -1;
+        long long rows[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) rows[k] = __shfl_sync(B2Q_FULL, at, (lane & 28) + k);
+        const bool b0 = lane & 1, b1 = lane & 2;
 #pragma unroll 1
         for (int x = 0; x < D; x += 32) {
-          uint32_t p[16];
+          uint4 v[4];
           if (it.nt > 0) {
             uint32_t o[32];
             pr_ld32(to + x, o);
             pr_wait_ld();
 #pragma unroll
-            for (int y = 0; y < 16; ++y) p[y] = el_pack2<T>(__uint_as_float(o[2 * y]) * inv, __uint_as_float(o[2 * y + 1]) * inv);
+            for (int k = 0; k < 4; ++k) {
+              uint32_t w[4];
+#pragma unroll
+              for (int y = 0; y < 4; ++y)
+                w[y] = el_pack2<T>(__uint_as_float(o[8 * k + 2 * y]) * inv, __uint_as_float(o[8 * k + 2 * y + 1]) * inv);
+              v[k] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
           } else {
 #pragma unroll
-            for (int y = 0; y < 16; ++y) p[y] = 0u;
+            for (int k = 0; k < 4; ++k) v[k] = make_uint4(0u, 0u, 0u, 0u);
           }
-          if (live) {
+          pr_swap(b0, 1, v[0], v[1]);
+          pr_swap(b0, 1, v[2], v[3]);
+          pr_swap(b1, 2, v[0], v[2]);
+          pr_swap(b1, 2, v[1], v[3]);
 #pragma unroll
-            for (int y = 0; y < 4; ++y)
-              reinterpret_cast<uint4*>(orow + x)[y] = make_uint4(p[4 * y], p[4 * y + 1], p[4 * y + 2], p[4 * y + 3]);
-          }
+          for (int k = 0; k < 4; ++k)
+            if (rows[k] >= 0) *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + rows[k] + x + (lane & 3) * 8) = v[k];
         }
         tc_fence_before();  // (the output's reads come before the next item's first product)
       }
+      it = nx;
     }
     if (!ok) *s_fail = 1;
   } else {
@@ -532,80 +544,84 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
         }
       }
     } else if (warp == 9) {
-      // ---- matrix instructions ----
-      if (lane == 0) {
-        constexpr uint32_t id_s = pr_idesc(BF, kPrN, false), id_o = pr_idesc(BF, D, true);
-        uint32_t ph = 0, land = 0, q_ph = 0, p_ph = 0;
-        int st = 0;
-        bool ok = true;
-        auto next = [&]() {
-          if (++st == NS) {
-            st = 0;
-            ph ^= 1;
-          }
-        };
-        auto scores = [&](int i, int ks) {  // S_i = Q_i K^T
-          const uint32_t q0 = smem_u32(qs + i * TB), k0 = smem_u32(ring + ks * TB);
+      // ---- matrix instructions: the whole warp keeps step, one thread issues ----
+      constexpr uint32_t id_s = pr_idesc(BF, kPrN, false), id_o = pr_idesc(BF, D, true);
+      const uint64_t q_desc = pr_desc(smem_u32(qs), 16), k_desc = pr_desc(smem_u32(ring), 16), v_desc = pr_desc(smem_u32(ring), CB);
+      uint32_t ph = 0, land = 0, q_ph = 0, p_ph = 0;
+      int st = 0;
+      bool ok = true;
+      auto next = [&]() {
+        if (++st == NS) {
+          st = 0;
+          ph ^= 1;
+        }
+      };
+      auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(B2Q_FULL, mbar_wait_bounded(bar, parity)) != 0; };
+      auto scores = [&](int i, int ks) {  // S_i = Q_i K^T
+        const uint64_t q = q_desc + (uint32_t)(i * (TB >> 4)), kd = k_desc + (uint32_t)(ks * (TB >> 4));
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint32_t o = (k >> 2) * CB + (k & 3) * 32;
-            pr_mma_ss(tmem + i * 128, pr_desc(q0 + o, 16), pr_desc(k0 + o, 16), id_s, k > 0);
-          }
-          pr_commit(&s_full[i]);
-        };
-        for (int round = 0; ok && round < rounds; ++round) {
-          PrItem it;
-          if (!item(round, it) || it.nt == 0) continue;
-          ok = mbar_wait_bounded(&full[st], ph);
-          for (int i = 0; ok && i < it.nq; ++i) {
-            ok = mbar_wait_bounded(&q_full[i], (q_ph >> i) & 1);
-            if (!ok) break;
-            q_ph ^= 1u << i;
-            tc_fence_after();
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t o = ((k >> 2) * CB + (k & 3) * 32) >> 4;
+          pr_mma_ss(tmem + i * 128, q + o, kd + o, id_s, k > 0);
+        }
+        pr_commit(&s_full[i]);
+      };
+      for (int round = 0; ok && round < rounds; ++round) {
+        PrItem it;
+        if (!item(round, it) || it.nt == 0) continue;
+        ok = wait(&full[st], ph);
+        for (int i = 0; ok && i < it.nq; ++i) {
+          ok = wait(&q_full[i], (q_ph >> i) & 1);
+          if (!ok) break;
+          q_ph ^= 1u << i;
+          tc_fence_after();
+          if (pr_elect()) {
             scores(i, st);
             if (it.nt == 1) pr_commit(&q_empty[i]);
           }
-          if (!ok) break;
-          pr_commit(&empty[st]);
+        }
+        if (!ok) break;
+        if (pr_elect()) pr_commit(&empty[st]);
+        next();
+        for (int j = 0; ok && j < it.nt; ++j) {
+          const bool more = j + 1 < it.nt;
+          const int sv = st;
+          ok = wait(&full[sv], ph);
+          if (ok && j >= it.kt_edge) {
+            ok = wait(&v_ok[sv], (land >> sv) & 1);
+            land ^= 1u << sv;
+          }
           next();
-          for (int j = 0; ok && j < it.nt; ++j) {
-            const bool more = j + 1 < it.nt;
-            const int sv = st;
-            ok = mbar_wait_bounded(&full[sv], ph);
-            if (ok && j >= it.kt_edge) {
-              ok = mbar_wait_bounded(&v_ok[sv], (land >> sv) & 1);
-              land ^= 1u << sv;
-            }
+          const int sk = st;
+          if (ok && more) {
+            ok = wait(&full[sk], ph);
             next();
-            const int sk = st;
-            if (ok && more) {
-              ok = mbar_wait_bounded(&full[sk], ph);
-              next();
-            }
-            for (int i = 0; ok && i < it.nq; ++i) {
-              ok = mbar_wait_bounded(&p_full[i], (p_ph >> i) & 1) && !*s_fail;
-              if (!ok) break;
-              p_ph ^= 1u << i;
-              tc_fence_after();
-              const uint32_t v0 = smem_u32(ring + sv * TB);
+          }
+          for (int i = 0; ok && i < it.nq; ++i) {
+            ok = wait(&p_full[i], (p_ph >> i) & 1) && !*s_fail;
+            if (!ok) break;
+            p_ph ^= 1u << i;
+            tc_fence_after();
+            if (pr_elect()) {
+              const uint64_t v = v_desc + (uint32_t)(sv * (TB >> 4));
 #pragma unroll
               for (int k = 0; k < kPrN / 16; ++k)
-                pr_mma_ts(tmem + 256 + i * D, tmem + i * 128 + k * 8, pr_desc(v0 + k * 2048, CB), id_o, j > 0 || k > 0);
+                pr_mma_ts(tmem + 256 + i * D, tmem + i * 128 + k * 8, v + ((k * 2048) >> 4), id_o, j > 0 || k > 0);
               if (more) scores(i, sk);
               else pr_commit(&o_full[i]);
               if (j + 2 == it.nt) pr_commit(&q_empty[i]);
             }
-            if (ok) {
-              pr_commit(&empty[sv]);
-              if (more) pr_commit(&empty[sk]);
-            }
+          }
+          if (ok && pr_elect()) {
+            pr_commit(&empty[sv]);
+            if (more) pr_commit(&empty[sk]);
           }
         }
-        if (!ok) {  // whatever was issued completes before the TMEM is freed
-          *s_fail = 1;
-          pr_commit(&done);
-          mbar_wait_bounded(&done, 0);
-        }
+      }
+      if (!ok) {  // whatever was issued completes before the TMEM is freed
+        *s_fail = 1;
+        if (pr_elect()) pr_commit(&done);
+        mbar_wait_bounded(&done, 0);
       }
     } else {
       // ---- value tiles that some row sees only in part ----

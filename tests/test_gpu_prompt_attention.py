@@ -43,7 +43,7 @@ def tiny(type_, v):
 
 
 def e_prob(type_):
-    return R.half_eps(TYPES[type_]) + (7.5e-5 if type_ == BF16 else 2.7e-6)
+    return R.half_eps(TYPES[type_])
 
 
 def check(engine, heads, kv, dim, type_, news, lens, scale=None, spread=1.0, seed=0, extra=0, **kw):
@@ -57,8 +57,7 @@ def check(engine, heads, kv, dim, type_, news, lens, scale=None, spread=1.0, see
     at = np.concatenate([[0], np.cumsum(lens)])
     rows = [[x[a:b].double().numpy() for a, b in zip(at[:-1], at[1:])] for x in (k, v)]
     # products of 16-bit values in f32 sums: 2^-19 of their magnitudes; the
-    # probabilities are rounded to the type, relative to a maximum that may lag, one
-    # in four after a polynomial that is off by 7.5e-5 (bf16) or 2.7e-6 (f16)
+    # probabilities are rounded to the type, relative to a maximum that may lag
     want, bound = R.attend(q[:T].double(), rows[0], rows[1], news, scale, TYPES[type_], 2.0 ** -19, e_prob(type_),
                            tiny(type_, v[:L]))
     if T:
