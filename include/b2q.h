@@ -412,7 +412,7 @@ typedef struct {
   int type;                          /* B2Q_F16 or B2Q_BF16: q, k, v and out */
   int n_seqs;                        /* at most 65535 */
   int n_q, n_kv;                     /* rows of q and out, rows of k and v */
-  int max_new;                       /* most queries of a sequence: chooses the tiling, never the result (0: unknown) */
+  int max_new;                       /* most queries of a sequence (0: unknown); never changes the result */
   const int32_t* q_start;            /* [n_seqs + 1], device */
   const int32_t* kv_start;           /* [n_seqs + 1], device */
 } b2q_prompt;

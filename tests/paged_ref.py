@@ -4,7 +4,7 @@ points document them), and of attention in f64 with an error bound of each
 output; and a pool of pages with the device arrays of a batch."""
 from __future__ import annotations
 
-import ctypes as C
+import functools
 import math
 
 import numpy as np
@@ -56,17 +56,24 @@ def values(code: np.ndarray, scale: np.ndarray) -> np.ndarray:
     return (b * scale.astype(np.float64)[..., None]).reshape(code.shape)
 
 
+@functools.lru_cache(maxsize=None)
+def _places(D: int):
+    """Where the 4-bit codes [16, D] of keys and values go: indices of half bytes."""
+    tok, dim = np.arange(16)[:, None], np.arange(D)[None, :]
+    b, t, n = dim // 32, dim % 32 // 8, dim % 8
+    keys = 2 * (tok * D // 2 + t * (D // 8) + b * 4 + n // 2) + n % 2
+    g, j = dim % 8, dim // 8
+    vals = 2 * (9 * D + tok // 8 * 4 * D + g * D // 2 + tok % 8 // 2 * (D // 8) + tok % 2 * (D // 16) + j // 2) + j % 2
+    return keys, vals
+
+
 def block_bytes(kc, ks, vc, vs) -> np.ndarray:
     """One block's bytes: kc, vc [16, D] codes, ks, vs [16, D / 32] f16."""
     D = kc.shape[1]
-    out = np.zeros(18 * D, np.uint8)
-    for tok in range(16):
-        for dim in range(D):
-            b, t, n = dim // 32, dim % 32 // 8, dim % 8
-            out[tok * D // 2 + t * (D // 8) + b * 4 + n // 2] |= kc[tok, dim] << (4 * (n % 2))
-            g, j = dim % 8, dim // 8
-            out[9 * D + tok // 8 * 4 * D + g * D // 2 + tok % 8 // 2 * (D // 8) + tok % 2 * (D // 16) + j // 2] |= (
-                vc[tok, dim] << (4 * (j % 2)))
+    half = np.zeros(36 * D, np.uint8)
+    keys, vals = _places(D)
+    half[keys], half[vals] = kc, vc
+    out = half[0::2] | half[1::2] << 4
     out[8 * D:9 * D] = np.ascontiguousarray(ks, np.float16).view(np.uint8).reshape(-1)
     out[17 * D:] = np.ascontiguousarray(vs, np.float16).view(np.uint8).reshape(-1)
     return out
