@@ -266,6 +266,11 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
     for (int i = 0; i < 8; ++i) s_poison[i] = 0;
     fence_mbar_init();
   }
+  if (warp == 8 && lane == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mq) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mk) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mv) : "memory");
+  }
   if (warp == 9) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512)
                  : "memory");

@@ -5,6 +5,8 @@
 // meet, and every call can be captured into a graph.
 #pragma once
 
+#include <atomic>
+
 #include "internal.h"
 #include "attn_paged.cuh"
 #include "attn_prompt.cuh"
@@ -116,14 +118,25 @@ static void by_dim(int D, F f) {
   else f(std::integral_constant<int, 128>());
 }
 
+// Lets a kernel take `bytes` of shared memory on the current device; asked
+// once per kernel and device (`done`: bits of the first 64).
+template <typename K>
+static cudaError_t allow_smem(K* kern, int bytes, int device, std::atomic<uint64_t>& done) {
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  const cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (err == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return err;
+}
+
 // CTAs of the paged attention: one per SM.
 static int paged_ctas(const b2q_engine* e) { return std::max(1, std::min(e->num_sms, kPgMaxCtas)); }
 static size_t paged_desc_bytes(int ctas) { return ((size_t)ctas * 2 * sizeof(PgDesc) + 255) / 256 * 256; }
 
 template <int D, int NG, bool QSPLIT, bool PSPLIT>
-static cudaError_t launch_paged(const PagedArgs& a, int ctas, cudaStream_t st) {
-  cudaError_t err = cudaFuncSetAttribute(attn_paged_kernel<D, NG, QSPLIT, PSPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         pg_ring_bytes(D, NG));
+static cudaError_t launch_paged(const PagedArgs& a, int ctas, int device, cudaStream_t st) {
+  static std::atomic<uint64_t> done{0};
+  cudaError_t err = allow_smem(attn_paged_kernel<D, NG, QSPLIT, PSPLIT>, pg_ring_bytes(D, NG), device, done);
   if (err != cudaSuccess) return err;
   cudaLaunchAttribute attr[1];
   cudaLaunchConfig_t cfg = dependent_launch((unsigned)ctas, pg_warps(NG) * 32, pg_ring_bytes(D, NG), st, attr);
@@ -162,9 +175,9 @@ static bool prompt_map_kv(CUtensorMap* m, const void* p, int64_t stride, int row
 }
 template <int D, int TYPE>
 static cudaError_t launch_prompt(const PromptArgs& a, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
-                                 unsigned grid, cudaStream_t st) {
-  cudaError_t err = cudaFuncSetAttribute(attn_prompt_kernel<D, TYPE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         pr_smem_bytes(D));
+                                 unsigned grid, int device, cudaStream_t st) {
+  static std::atomic<uint64_t> done{0};
+  cudaError_t err = allow_smem(attn_prompt_kernel<D, TYPE>, pr_smem_bytes(D), device, done);
   if (err != cudaSuccess) return err;
   cudaLaunchAttribute attr[1];
   const cudaLaunchConfig_t cfg = dependent_launch(grid, kPrThreads, pr_smem_bytes(D), st, attr);
@@ -341,9 +354,9 @@ b2q_status b2q_attn_paged_dev(b2q_engine* e, const b2q_kv_config* cfg, const b2q
   const bool split = ot == kElF32;
   cudaError_t err = cudaSuccess;
   by_dim(D, [&](auto d) {
-    if (wide) err = split ? launch_paged<d(), 2, false, true>(a, ctas, st) : launch_paged<d(), 2, false, false>(a, ctas, st);
-    else if (qt == kElF32) err = split ? launch_paged<d(), 1, true, true>(a, ctas, st) : launch_paged<d(), 1, true, false>(a, ctas, st);
-    else err = split ? launch_paged<d(), 1, false, true>(a, ctas, st) : launch_paged<d(), 1, false, false>(a, ctas, st);
+    if (wide) err = split ? launch_paged<d(), 2, false, true>(a, ctas, e->device, st) : launch_paged<d(), 2, false, false>(a, ctas, e->device, st);
+    else if (qt == kElF32) err = split ? launch_paged<d(), 1, true, true>(a, ctas, e->device, st) : launch_paged<d(), 1, true, false>(a, ctas, e->device, st);
+    else err = split ? launch_paged<d(), 1, false, true>(a, ctas, e->device, st) : launch_paged<d(), 1, false, false>(a, ctas, e->device, st);
   });
   launch_counted(e, 2);
   return err == cudaSuccess ? B2Q_OK : cuda_error(err, what);
@@ -408,8 +421,8 @@ b2q_status b2q_attn_prompt_dev(b2q_engine* e, const b2q_prompt* p, const void* q
   cudaStream_t st = stream ? (cudaStream_t)stream : e->stream;
   cudaError_t err = cudaSuccess;
   by_dim(D, [&](auto d) {
-    err = t == kElF16 ? launch_prompt<d(), kElF16>(a, mq, mk, mv, grid, st)
-                      : launch_prompt<d(), kElBF16>(a, mq, mk, mv, grid, st);
+    err = t == kElF16 ? launch_prompt<d(), kElF16>(a, mq, mk, mv, grid, e->device, st)
+                      : launch_prompt<d(), kElBF16>(a, mq, mk, mv, grid, e->device, st);
   });
   launch_counted(e, 1);
   return err == cudaSuccess ? B2Q_OK : cuda_error(err, what);
