@@ -3,17 +3,20 @@
 // and l keys attends the keys j <= i + l - n.
 //
 // S = Q K^T and O += P V run on the 5th-generation tensor cores with their
-// accumulators in TMEM.  An item is two tiles of 128 query rows of a K/V head (one
-// where that fills the GPU better); a row is a (token, head) pair, the G heads of a K/V
-// head side by side, so that a short prompt fills a tile and each K/V tile is
-// fetched once for all of them.  Over the key tiles (128 keys, K and V by TMA into
-// a ring of 32 KB stages at D = 128) the two row tiles take turns: while one's
-// scores go through the softmax the matrix unit works on the other's.  One CTA an
-// SM goes from item to item, the next item's loads and first scores under the
+// accumulators in TMEM.  An item is two tiles of 128 query rows of a K/V head; a
+// row is a (token, head) pair, the G heads of a K/V head side by side, so that a
+// short prompt fills a tile and each K/V tile is fetched once for all of them.
+// Over the key tiles (128 keys, K and V by TMA into a ring of 32 KB stages at D =
+// 128) the two row tiles take turns: while one's scores go through the softmax the
+// matrix unit works on the other's.  Where that leaves SMs without an item, an
+// item is one row tile, and the CTA's halves take its key tiles in turn, each with a
+// running softmax and an output of its own, joined at the end (HALVES).  One CTA
+// an SM goes from item to item, the next item's loads and first scores under the
 // last one's epilogue.
-//   warps 0-3, 4-7  softmax of row tile 0 / 1: a thread owns a row, reads its
-//                   128 scores out of TMEM, and writes the probabilities over
-//                   them in the 16-bit type, where the P V product reads them;
+//   warps 0-3, 4-7  softmax of row tile 0 / 1, or of even / odd key tiles: a
+//                   thread owns a row, reads its 128 scores out of TMEM, and
+//                   writes the probabilities over them in the 16-bit type, where
+//                   the P V product reads them;
 //   warp 8          TMA;   warp 9  issues the matrix instructions;
 //   warps 10, 11    look over the value tiles that some row sees only in part.
 // What bounds it: the matrix unit (16 instructions of 64 cycles for each row tile
@@ -23,10 +26,12 @@
 // the issuing warp converged, with one elected thread, 981 -> 910 us (a branch on the
 // lane moved every descriptor between register files); the next item's geometry
 // under the last product and stores of 64 consecutive bytes, 910 -> 893 (16 ragged
-// prompts 172 -> 157).  Tried on the 984 us form: a quarter of the exponentials by a
-// polynomial on the FMA units, 1040; two threads to a row, 1027; key tiles of 64 with two
-// score buffers, 1270 (a score product of 64 keys takes as long as one of
-// 128: its A operand's trip from shared memory).
+// prompts 172 -> 157).  That is a burst; where the power cap holds the clock at 1.6
+// to 1.7 GHz it takes 1046.  16 tokens behind 2048, 32 heads over 8: 23 us in halves,
+// 32.5 without (512 tokens behind 2048: 29 and 39).  Tried on the 984 us form: a
+// quarter of the exponentials by a polynomial on the FMA units, 1040; two threads to
+// a row, 1027; key tiles of 64 with two score buffers, 1270 (a score product of 64
+// keys takes as long as one of 128: its A operand's trip from shared memory).
 // The running maximum moves only when a row's grows by more than 2^8: until
 // then probabilities up to 2^15 serve as well (they start at 2^7 for the largest,
 // out of f16's subnormals), and the output in TMEM needs no rescaling.  When it
@@ -229,7 +234,7 @@ struct PrItem {
 
 constexpr int kPrSeqs = 192;  // sequences whose offsets are copied to shared memory
 
-template <int D, int TYPE>
+template <int D, int TYPE, bool HALVES>
 __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid_constant__ PromptArgs a,
                                                                     const __grid_constant__ CUtensorMap mq,
                                                                     const __grid_constant__ CUtensorMap mk,
@@ -239,7 +244,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
   constexpr int NC = D / 64;
   constexpr bool BF = TYPE == kElBF16;
   extern __shared__ uint8_t pr_smem[];
-  __shared__ uint64_t q_full[2], q_empty[2], full[NS], empty[NS], v_land[NS], v_ok[NS], s_full[2], p_full[2], o_full[2], done;
+  __shared__ uint64_t q_full[2], q_empty[2], full[NS], empty[NS], v_land[NS], v_ok[NS], s_full[2], p_full[2], o_full[2], x_full, o_free, done;
   __shared__ uint32_t s_tmem;
   __shared__ int s_fail_, s_poison_[8], s_q[kPrSeqs + 1], s_k[kPrSeqs + 1];
   volatile int *s_fail = &s_fail_, *s_poison = s_poison_;
@@ -261,6 +266,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
       mbar_init(&v_land[i], 1);
       mbar_init(&v_ok[i], 2);
     }
+    mbar_init(&x_full, 8);
+    mbar_init(&o_free, 8);
     mbar_init(&done, 1);
     *s_fail = 0;
     for (int i = 0; i < 8; ++i) s_poison[i] = 0;
@@ -293,7 +300,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
   // q_start[s] / bt + s on (increasing in s, and enough for it).  CTA b takes b,
   // then goes back and forth: late slots, which see the most keys, come first,
   // and what one round gives a CTA too much the next takes from it ----
-  const int bt = a.nq * a.tpt;
+  constexpr int NQ = HALVES ? 1 : 2, step = HALVES ? 2 : 1;  // row tiles of an item; from a half's key tile to its next
+  const int bt = NQ * a.tpt;
   auto item = [&](int round, PrItem& it) {  // false: nothing to do
     const int x = round * (int)gridDim.x + ((round & 1) ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x);
     if (x >= a.items) return false;
@@ -322,7 +330,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
     it.n = qe - qa;
     it.l = ke - ka;
     it.tok0 = (int)tok0;
-    it.nq = a.nq == 2 && it.tok0 + a.tpt < it.n ? 2 : 1;
+    it.nq = !HALVES && it.tok0 + a.tpt < it.n ? 2 : 1;
     const int diff = it.l - it.n;  // token i attends the keys up to i + diff
     const int kmax = max(0, min(it.n, it.tok0 + bt) + diff);
     it.nt = (kmax + kPrN - 1) / kPrN;
@@ -334,14 +342,15 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
 
   if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-    // ---- softmax of row tile i ----
-    const int i = warp >> 2, r = threadIdx.x & 127;
+    // ---- softmax of row tile i, or of every second key tile ----
+    const int i = warp >> 2, ir = HALVES ? 0 : i, r = threadIdx.x & 127;
+    float2* s_stat = reinterpret_cast<float2*>(qs + TB);  // [2][2][128] (halves: no second query tile): reference, sum
     const int tr = fdiv(r, a.d_gp), hr = r - tr * a.gp;  // the row's token and head within the tile
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + lane_base + i * 128, to = tmem + lane_base + 256 + i * D;
     const float c = a.scale * 1.4426950408889634f;
     const f2 c2 = f2_of(c, c);
-    uint32_t s_ph = 0, o_ph = 0;
+    uint32_t s_ph = 0, o_ph = 0, x_ph = 0;  // (o_ph: a bit for each half)
     int count = 0;  // items with key tiles, of either row tile
     bool ok = true;
     int round = -1;
@@ -349,7 +358,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
       while (++round < rounds) {
         if (!item(round, it)) continue;
         if (it.nt > 0) ++count;
-        if (i < it.nq) return true;
+        if (ir < it.nq) return true;
       }
       return false;
     };
@@ -357,12 +366,12 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
     bool more = next_item(it);
     while (ok && more) {
       const int mine = count;  // (the item's)
-      const int diff = it.l - it.n, tok = it.tok0 + i * a.tpt + tr, h = it.hoff + hr;
+      const int diff = it.l - it.n, tok = it.tok0 + ir * a.tpt + tr, h = it.hoff + hr;
       const bool live = tr < a.tpt && tok < it.n && h < a.G;
       const int lim = min(tok + diff, it.l - 1);          // the row's last key
-      const int edge = it.tok0 + i * a.tpt + diff;        // the tile's first token's
+      const int edge = it.tok0 + ir * a.tpt + diff;       // the tile's first token's
       float ref = -INFINITY, sum = 0.0f;                  // (scores times c)
-      for (int j = 0; j < it.nt; ++j) {
+      for (int j = HALVES ? i : 0; j < it.nt; j += step) {
         ok = __all_sync(B2Q_FULL, mbar_wait_bounded(&s_full[i], s_ph)) && !*s_fail;
         if (!ok) break;
         s_ph ^= 1;
@@ -392,7 +401,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
           const float al = move ? (ref == -INFINITY ? 0.0f : pr_exp2(ref - m)) : 1.0f;
           if (move) ref = m;
           sum *= al;
-          if (j > 0) {
+          if (j >= step) {
 #pragma unroll 1
             for (int x = 0; x < D; x += 32) {
               uint32_t o[32];
@@ -436,15 +445,37 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
       // ---- epilogue: the next item's geometry under the last product ----
       PrItem nx;
       more = next_item(nx);
+      float w0 = 1.0f, w1 = 0.0f;  // weights of the halves' outputs
       if (it.nt > 0) {
-        ok = __all_sync(B2Q_FULL, mbar_wait_bounded(&o_full[i], o_ph)) && !*s_fail;
-        if (!ok) break;
+        // (in halves both outputs; a second one where there are two key tiles)
+        ok = __all_sync(B2Q_FULL, mbar_wait_bounded(&o_full[ir], o_ph & 1)) && !*s_fail;
         o_ph ^= 1;
+        if (HALVES && ok && it.nt > 1) {
+          ok = __all_sync(B2Q_FULL, mbar_wait_bounded(&o_full[1], o_ph >> 1)) && !*s_fail;
+          o_ph ^= 2;
+        }
+        if (!ok) break;
         tc_fence_after();
+        if (HALVES) {
+          // both halves meet at each item, so that the two places for what they
+          // tell one another (x_ph) are free again when they are next written
+          float2* stat = s_stat + x_ph * 256;
+          stat[128 * i + r] = make_float2(ref, sum);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&x_full);
+          ok = __all_sync(B2Q_FULL, mbar_wait_bounded(&x_full, x_ph)) && !*s_fail;
+          if (!ok) break;
+          x_ph ^= 1;
+          const float2 st0 = stat[r], st1 = stat[128 + r];
+          const float top = fmaxf(st0.x, st1.x);
+          w0 = st0.x == -INFINITY ? 0.0f : pr_exp2(st0.x - top);
+          w1 = st1.x == -INFINITY ? 0.0f : pr_exp2(st1.x - top);
+          sum = w0 * st0.y + w1 * st1.y;
+        }
       }
       if (it.nt > 0 && s_poison[mine & 7] == mine) {
         for (int y = 0; y < 32; ++y) {
-          if (!__shfl_sync(B2Q_FULL, (int)live, y)) continue;
+          if (!__shfl_sync(B2Q_FULL, (int)live, y) || (HALVES && (y & 1) != i)) continue;
           const int tk = __shfl_sync(B2Q_FULL, tok, y), hh = __shfl_sync(B2Q_FULL, h, y);
           prompt_row_slow<D, T>(a, it.qa + tk, it.kvh * a.G + hh, it.ka, tk + diff);
         }
@@ -457,13 +488,25 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
 #pragma unroll
         for (int k = 0; k < 4; ++k) rows[k] = __shfl_sync(B2Q_FULL, at, (lane & 28) + k);
         const bool b0 = lane & 1, b1 = lane & 2;
+        const int xa = HALVES ? i * (D / 2) : 0, xe = HALVES ? xa + D / 2 : D;
 #pragma unroll 1
-        for (int x = 0; x < D; x += 32) {
+        for (int x = xa; x < xe; x += 32) {
           uint4 v[4];
           if (it.nt > 0) {
             uint32_t o[32];
-            pr_ld32(to + x, o);
+            pr_ld32((HALVES ? tmem + lane_base + 256 : to) + x, o);
             pr_wait_ld();
+            if (HALVES) {
+#pragma unroll
+              for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * w0);
+              if (it.nt > 1) {
+                uint32_t o1[32];
+                pr_ld32(tmem + lane_base + 256 + D + x, o1);
+                pr_wait_ld();
+#pragma unroll
+                for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(fmaf(__uint_as_float(o1[y]), w1, __uint_as_float(o[y])));
+              }
+            }
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               uint32_t w[4];
@@ -486,13 +529,17 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
         }
         tc_fence_before();  // (the output's reads come before the next item's first product)
       }
+      if (HALVES && it.nt > 0) {  // (which reads no probabilities of this half)
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&o_free);
+      }
       it = nx;
     }
     if (!ok) *s_fail = 1;
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 8) {
-      // ---- TMA: Q0, K0, Q1, V0, K1, V1, ... ----
+      // ---- TMA: Q0, K0, Q1, V0, K1, V1, ...; in halves Q0, K0, K1, V0, K2, V1, ... ----
       if (lane == 0) {
         const uint32_t qbytes = (uint32_t)(a.tpt * a.gp * 128 * NC);
         uint32_t ph = 0, land = 0, q_ph = 0;        // phases: of the ring, bits per stage, bits per row tile
@@ -519,11 +566,13 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
             // lookers follow without the uses of the ring before them; their stage's
             // full barrier is passed at once.  v_land and v_ok are per stage, so that
             // neither can run a phase ahead of whom it wakes.
-            const bool look = (x & 1) && (x >> 1) >= it.kt_edge;
+            const bool value = !HALVES ? x & 1 : x == 2 * it.nt - 1 || (x > 0 && (x & 1) == 0);
+            const int tile = !HALVES ? x >> 1 : x == 2 * it.nt - 1 ? it.nt - 1 : (x & 1) ? (x + 1) >> 1 : max(0, (x >> 1) - 1);
+            const bool look = value && tile >= it.kt_edge;
             uint64_t* bar = look ? &v_land[st] : &full[st];
             mbar_arrive_expect_tx(bar, (uint32_t)TB);
             for (int cnk = 0; cnk < NC; ++cnk)
-              tma_load_3d(ring + st * TB + cnk * CB, (x & 1) ? &mv : &mk, cnk * 64, it.kvh, it.ka + (x >> 1) * kPrN, bar);
+              tma_load_3d(ring + st * TB + cnk * CB, value ? &mv : &mk, cnk * 64, it.kvh, it.ka + tile * kPrN, bar);
             if (look) {
               mbar_arrive(&full[st]);
               land ^= 1u << st;
@@ -563,7 +612,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
       };
       auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(B2Q_FULL, mbar_wait_bounded(bar, parity)) != 0; };
       auto scores = [&](int i, int ks) {  // S_i = Q_i K^T
-        const uint64_t q = q_desc + (uint32_t)(i * (TB >> 4)), kd = k_desc + (uint32_t)(ks * (TB >> 4));
+        const uint64_t q = q_desc + (uint32_t)((HALVES ? 0 : i) * (TB >> 4)), kd = k_desc + (uint32_t)(ks * (TB >> 4));
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           const uint32_t o = ((k >> 2) * CB + (k & 3) * 32) >> 4;
@@ -571,25 +620,31 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
         }
         pr_commit(&s_full[i]);
       };
+      uint32_t o_ph = 1;  // of o_free: the first item waits for none
       for (int round = 0; ok && round < rounds; ++round) {
         PrItem it;
         if (!item(round, it) || it.nt == 0) continue;
-        ok = wait(&full[st], ph);
-        for (int i = 0; ok && i < it.nq; ++i) {
-          ok = wait(&q_full[i], (q_ph >> i) & 1);
+        // the first scores: of both row tiles with the first keys, or of the one
+        // with the first two
+        const int ns = HALVES ? min(2, it.nt) : it.nq;
+        for (int i = 0; ok && i < ns; ++i) {
+          if (i == 0 || HALVES) ok = wait(&full[st], ph);
+          if (ok && (i == 0 || !HALVES)) {
+            ok = wait(&q_full[i], (q_ph >> i) & 1);
+            q_ph ^= 1u << i;
+          }
           if (!ok) break;
-          q_ph ^= 1u << i;
           tc_fence_after();
+          const bool last = HALVES || i + 1 == ns;  // the keys' last use
           if (pr_elect()) {
             scores(i, st);
-            if (it.nt == 1) pr_commit(&q_empty[i]);
+            if (it.nt == (HALVES ? i + 1 : 1)) pr_commit(&q_empty[HALVES ? 0 : i]);
+            if (last) pr_commit(&empty[st]);
           }
+          if (last) next();
         }
-        if (!ok) break;
-        if (pr_elect()) pr_commit(&empty[st]);
-        next();
         for (int j = 0; ok && j < it.nt; ++j) {
-          const bool more = j + 1 < it.nt;
+          const bool more = j + step < it.nt;
           const int sv = st;
           ok = wait(&full[sv], ph);
           if (ok && j >= it.kt_edge) {
@@ -602,19 +657,24 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
             ok = wait(&full[sk], ph);
             next();
           }
-          for (int i = 0; ok && i < it.nq; ++i) {
+          if (ok && HALVES && j == 0) {  // both halves have read the last item's outputs
+            ok = wait(&o_free, o_ph);
+            o_ph ^= 1;
+          }
+          const int ie = HALVES ? (j & 1) + 1 : it.nq;
+          for (int i = HALVES ? j & 1 : 0; ok && i < ie; ++i) {
             ok = wait(&p_full[i], (p_ph >> i) & 1) && !*s_fail;
             if (!ok) break;
             p_ph ^= 1u << i;
             tc_fence_after();
             if (pr_elect()) {
-              const uint64_t v = v_desc + (uint32_t)(sv * (TB >> 4));
+              const uint64_t v = v_desc + (uint32_t)(sv * (TB >> 4));  // O_i (+)= P_i V
 #pragma unroll
               for (int k = 0; k < kPrN / 16; ++k)
-                pr_mma_ts(tmem + 256 + i * D, tmem + i * 128 + k * 8, v + ((k * 2048) >> 4), id_o, j > 0 || k > 0);
+                pr_mma_ts(tmem + 256 + i * D, tmem + i * 128 + k * 8, v + ((k * 2048) >> 4), id_o, j >= step || k > 0);
               if (more) scores(i, sk);
               else pr_commit(&o_full[i]);
-              if (j + 2 == it.nt) pr_commit(&q_empty[i]);
+              if (j + 1 + step == it.nt) pr_commit(&q_empty[HALVES ? 0 : i]);
             }
           }
           if (ok && pr_elect()) {
@@ -639,7 +699,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
         if (!item(round, it) || it.nt == 0) continue;
         ++count;
         for (int j = it.kt_edge; j < it.nt; ++j) {
-          const int st = (x0 + 2 * j + 1) % NS;
+          const int st = (x0 + (HALVES && j + 1 < it.nt ? 2 * j + 2 : 2 * j + 1)) % NS;
           ok = __all_sync(B2Q_FULL, mbar_wait_bounded(&v_land[st], (land >> st) & 1)) && !*s_fail;
           if (!ok) break;
           land ^= 1u << st;

@@ -173,15 +173,15 @@ static bool prompt_map_kv(CUtensorMap* m, const void* p, int64_t stride, int row
   const cuuint32_t box[3] = {64u, 1u, (cuuint32_t)kPrN};
   return prompt_map(m, type, 3, p, dims, strides, box);
 }
-template <int D, int TYPE>
+template <int D, int TYPE, bool HALVES>
 static cudaError_t launch_prompt(const PromptArgs& a, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
                                  unsigned grid, int device, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
-  cudaError_t err = allow_smem(attn_prompt_kernel<D, TYPE>, pr_smem_bytes(D), device, done);
+  cudaError_t err = allow_smem(attn_prompt_kernel<D, TYPE, HALVES>, pr_smem_bytes(D), device, done);
   if (err != cudaSuccess) return err;
   cudaLaunchAttribute attr[1];
   const cudaLaunchConfig_t cfg = dependent_launch(grid, kPrThreads, pr_smem_bytes(D), st, attr);
-  return cudaLaunchKernelEx(&cfg, attn_prompt_kernel<D, TYPE>, a, mq, mk, mv);
+  return cudaLaunchKernelEx(&cfg, attn_prompt_kernel<D, TYPE, HALVES>, a, mq, mk, mv);
 }
 
 }  // namespace b2q
@@ -406,7 +406,9 @@ b2q_status b2q_attn_prompt_dev(b2q_engine* e, const b2q_prompt* p, const void* q
   if (!prompt_map_q(&mq, a, D, t) || !prompt_map_kv(&mk, a.k, a.k_stride, a.n_kv, a.KV, D, t) ||
       !prompt_map_kv(&mv, a.v, a.v_stride, a.n_kv, a.KV, D, t))
     return set_error(B2Q_ECUDA, "%s: cuTensorMapEncodeTiled failed", what);
-  // two row tiles to an item, one where that still does not give every SM an item
+  // two row tiles to an item; one, in halves, where those are no more than the SMs
+  // (16 tokens behind 2048: 23 us, 32 with room for a second row tile; with more items
+  // than SMs two rounds of half the length gain nothing and load the keys twice)
   const int64_t hc = (int64_t)a.KV * a.chunks;
   a.nq = ((int64_t)(a.n_q / a.tpt) + a.n_seqs) * hc <= e->num_sms ? 1 : 2;
   const int64_t slots = (int64_t)(a.n_q / (a.nq * a.tpt)) + a.n_seqs;
@@ -421,8 +423,12 @@ b2q_status b2q_attn_prompt_dev(b2q_engine* e, const b2q_prompt* p, const void* q
   cudaStream_t st = stream ? (cudaStream_t)stream : e->stream;
   cudaError_t err = cudaSuccess;
   by_dim(D, [&](auto d) {
-    err = t == kElF16 ? launch_prompt<d(), kElF16>(a, mq, mk, mv, grid, e->device, st)
-                      : launch_prompt<d(), kElBF16>(a, mq, mk, mv, grid, e->device, st);
+    if (a.nq == 1)
+      err = t == kElF16 ? launch_prompt<d(), kElF16, true>(a, mq, mk, mv, grid, e->device, st)
+                        : launch_prompt<d(), kElBF16, true>(a, mq, mk, mv, grid, e->device, st);
+    else
+      err = t == kElF16 ? launch_prompt<d(), kElF16, false>(a, mq, mk, mv, grid, e->device, st)
+                        : launch_prompt<d(), kElBF16, false>(a, mq, mk, mv, grid, e->device, st);
   });
   launch_counted(e, 1);
   return err == cudaSuccess ? B2Q_OK : cuda_error(err, what);

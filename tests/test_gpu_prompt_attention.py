@@ -17,11 +17,27 @@ def rand(shape, seed, type_, spread=1.0):
     return (torch.randn(*shape, generator=g) * spread).to(TYPES[type_])
 
 
+PAD = 0
+
+
+@pytest.fixture(autouse=True, params=[0, 20000], ids=["few rows", "many rows"])
+def pad(request):
+    """Rows behind the last sequence: with many of them the call takes two row
+    tiles at a time instead of one in two halves."""
+    global PAD
+    PAD = request.param
+    yield
+    PAD = 0
+
+
 def run_prompt(engine, heads, kv, dim, type_, news, lens, q, k, v, scale, max_new=None, strides=None, n_q=None, stream=None, out=None):
     from hf_llm_b200 import paged
     qs = torch.tensor(np.concatenate([[0], np.cumsum(news)]), dtype=torch.int32).cuda()
     ks = torch.tensor(np.concatenate([[0], np.cumsum(lens)]), dtype=torch.int32).cuda()
     q, k, v = (x if x.is_cuda else x.cuda() for x in (q, k, v))
+    rows = q.shape[0]
+    if PAD and out is None and strides is None:
+        q = torch.cat([q, torch.full((PAD,) + tuple(q.shape[1:]), float("nan"), dtype=q.dtype, device="cuda")])
     n_q = q.shape[0] if n_q is None else n_q
     if out is None:
         out = torch.full((q.shape[0], heads, dim), 7.0, dtype=TYPES[type_], device="cuda")
@@ -32,7 +48,8 @@ def run_prompt(engine, heads, kv, dim, type_, news, lens, q, k, v, scale, max_ne
     engine.attn_prompt_dev(p, q.data_ptr(), st[0], k.data_ptr(), st[1], v.data_ptr(), st[2], scale, out.data_ptr(),
                            stream or torch.cuda.current_stream().cuda_stream or 1)
     torch.cuda.synchronize()
-    return out
+    assert (out[rows:] == 7.0).all()
+    return out[:rows]
 
 
 def tiny(type_, v):
@@ -213,7 +230,7 @@ def test_captured_and_replayed_with_other_lengths(engine, pkg):
         with torch.cuda.stream(s):
             g.replay()
         torch.cuda.synchronize()
-        want = run_prompt(engine, 4, 2, 64, BF16, [mid, end - mid], [mid, end - mid], q, k, v, 0.125)
+        want = run_prompt(engine, 4, 2, 64, BF16, [mid, end - mid], [mid, end - mid], q, k, v, 0.125, out=torch.full_like(out, 7.0))
         assert torch.equal(out, want)
 
 
