@@ -145,6 +145,13 @@ __device__ __forceinline__ int pg_per(const PagedArgs& a, const PgSeq& q) {
 }
 __device__ __forceinline__ int pg_units(const PagedArgs& a, const PgSeq& q) { return q.nrb * a.b.KV * pg_per(a, q); }
 
+// Units of a warp's lanes (each below 2^31) in all, at most kPgFull.
+constexpr unsigned kPgFull = 0x7fffffffu;
+__device__ __forceinline__ unsigned pg_sum(unsigned v) {
+  const unsigned lo = __reduce_add_sync(B2Q_FULL, v & 0xffffu), hi = __reduce_add_sync(B2Q_FULL, v >> 16);
+  return hi >= 0x8000u ? kPgFull : min((hi << 16) + lo, kPgFull);
+}
+
 // A place in the line: block blk of item (seq, sub), sub = row block * KV + K/V
 // head.  The end of the line is sequence n_seqs.
 struct PgAt {
@@ -318,16 +325,20 @@ __global__ void __launch_bounds__(PgThreads<NG>::value, 1) attn_paged_kernel(con
   if (nch > 1) {
     for (int c = warp; c < nch; c += W) {
       const int s = c * kPgChunk + lane;
-      const int w = __reduce_add_sync(B2Q_FULL, s < a.b.n_seqs ? pg_units(a, pg_seq<NG>(a, s)) : 0);
-      if (lane == 0) sums[c] = w;
+      const unsigned w = pg_sum(s < a.b.n_seqs ? pg_units(a, pg_seq<NG>(a, s)) : 0);
+      if (lane == 0) sums[c] = (int)w;
     }
     __syncthreads();
-    for (int c = lane; c < nch; c += 32) v0 += sums[c];
+    for (int c = lane; c < nch; c += 32) v0 = (int)min((unsigned)v0 + (unsigned)sums[c], kPgFull);
   } else if (lane < a.b.n_seqs) {  // every warp has all of them in its lanes
     q0 = pg_seq<NG>(a, lane);
     v0 = pg_units(a, q0);
   }
-  const unsigned total = (unsigned)__reduce_add_sync(B2Q_FULL, v0);
+  unsigned total = pg_sum(v0);
+  if (total == kPgFull) {  // offsets that go up and down give more rows than there are: nothing is done
+    if (threadIdx.x == 0) kv_batch_error();
+    total = 0;
+  }
   const unsigned nc = min(gridDim.x, (total + W * kPgMin - 1) / (W * kPgMin));
   const bool working = blockIdx.x < nc;
   if (working) {

@@ -88,7 +88,8 @@ __device__ __noinline__ void prompt_row_slow(const PromptArgs& a, int tok, int h
 #pragma unroll
     for (int e = 0; e < E; ++e) s = fmaf(q[e], el_f(kr[lane + 32 * e]), s);
     s = warp_sum(s);
-    const float nm = fmaxf(m, s), al = expf(m - nm), p = expf(s - nm);
+    const float nm = fmaxf(m, s);  // (a score of -inf has no weight, one that is NaN shows)
+    const float al = m == -INFINITY ? 0.0f : expf(m - nm), p = s == -INFINITY ? 0.0f : expf(s - nm);
     m = nm;
     sum = sum * al + p;
 #pragma unroll

@@ -315,7 +315,7 @@ b2q_status b2q_attn_paged_dev(b2q_engine* e, const b2q_kv_config* cfg, const b2q
   if (!pages || !aligned16(pages)) return set_error(B2Q_EINVAL, "%s: pages must be a 16-byte aligned pointer", what);
   if ((int64_t)batch->n_tokens * cfg->n_heads > (1 << 30))
     return set_error(B2Q_EINVAL, "%s: %d tokens of %d heads in one call", what, batch->n_tokens, cfg->n_heads);
-  if (!(scale > 0.0f && scale <= 3.0e38f)) return set_error(B2Q_EINVAL, "%s: scale must be positive and finite", what);
+  if (!(scale > 0.0f && scale <= 1e30f)) return set_error(B2Q_EINVAL, "%s: scale must be positive and at most 1e30", what);
   const size_t need = b2q_attn_paged_work_bytes(e, cfg, batch);
   if (!work || !aligned16(work) || work_bytes < need)
     return set_error(B2Q_EINVAL, "%s: a workspace of %zu bytes is needed (%zu given)", what, need, work_bytes);
@@ -379,7 +379,7 @@ b2q_status b2q_attn_prompt_dev(b2q_engine* e, const b2q_prompt* p, const void* q
   if (s == B2Q_OK && p->n_kv) s = check_rows(what, "k", k, k_stride, (int64_t)p->n_kv_heads * D, t);
   if (s == B2Q_OK && p->n_kv) s = check_rows(what, "v", v, v_stride, (int64_t)p->n_kv_heads * D, t);
   if (s != B2Q_OK) return s;
-  if (!(scale > 0.0f && scale <= 3.0e38f)) return set_error(B2Q_EINVAL, "%s: scale must be positive and finite", what);
+  if (!(scale > 0.0f && scale <= 1e30f)) return set_error(B2Q_EINVAL, "%s: scale must be positive and at most 1e30", what);
   DeviceGuard dev(e->device);
   if (dev.err != cudaSuccess) return cuda_error(dev.err, what);
   PromptArgs a;

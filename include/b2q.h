@@ -395,7 +395,9 @@ b2q_status b2q_kv_gather_dev(b2q_engine* eng, const b2q_kv_config* cfg, const b2
  * positions j up to the token's own.  A token without keys gives zeros.
  * Sums and the softmax in f32; f32 queries are carried as two f16 parts
  * (~2^-22), and so is a probability times its value's scale where out is f32;
- * for 16-bit outputs that product is rounded once, to f16.  out [n_tokens][n_heads * head_dim] contiguous.
+ * for 16-bit outputs that product is rounded once, to f16.  0 < scale <=
+ * 1e30.  out [n_tokens][n_heads * head_dim] contiguous.  Offsets that go up and
+ * down until the sequences' rows are many times the batch's: nothing is done.
  * `work`: at least b2q_attn_paged_work_bytes() (16-byte aligned; no initial
  * contents needed). */
 size_t b2q_attn_paged_work_bytes(const b2q_engine* eng, const b2q_kv_config* cfg, const b2q_kv_batch* batch);
@@ -419,7 +421,7 @@ typedef struct {
 
 /* Causal attention of packed prompts, query heads grouped as above.  out
  * [n_q][n_heads * head_dim] contiguous; rows from q_start[n_seqs] on are left
- * as they are, queries without keys give zeros.  Scores, sums and outputs are
+ * as they are, queries without keys give zeros.  0 < scale <= 1e30.  Scores, sums and outputs are
  * accumulated in f32, the probabilities rounded to `type`. */
 b2q_status b2q_attn_prompt_dev(b2q_engine* eng, const b2q_prompt* p, const void* q, int64_t q_stride, const void* k,
                                int64_t k_stride, const void* v, int64_t v_stride, float scale, void* out, void* stream);

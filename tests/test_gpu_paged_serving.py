@@ -261,6 +261,32 @@ def test_rows_further_apart_than_32_bits_of_elements(engine, pkg):
     engine.check_device_error()
 
 
+def test_offsets_that_count_the_rows_again_and_again(engine, pkg):
+    """300 of 600 sequences claim all rows with 2^22 keys each: above 2^31 units of
+    work, which is reported and not begun."""
+    from hf_llm_b200 import paged
+    from hf_llm_b200._lib import B2QError, EINVAL
+    H, D, T, S, P, mp = 4, 64, 64, 600, 4096, 1024
+    cfg = paged.kv_config(H, H, D, R.Q4_0, P, 1, mp)
+    start = torch.tensor([0, T] * (S // 2) + [0], dtype=torch.int32).cuda()
+    lens = torch.full((S,), mp * P, dtype=torch.int32).cuda()
+    table = torch.full((S, mp), -1, dtype=torch.int32).cuda()
+    pages = torch.empty(paged.page_bytes(cfg), dtype=torch.uint8, device="cuda")
+    b = paged.kv_batch(S, T, 1, start.data_ptr(), lens.data_ptr(), table.data_ptr())
+    assert 300 * (T // 8) * H * (mp * P // 16 + 5) > 2 ** 31
+    q = rand((T, H, D), 1).cuda()
+    out = torch.full_like(q, 7.0)
+    work = torch.empty(engine.attn_paged_work_bytes(cfg, b), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    engine.attn_paged_dev(cfg, b, q.data_ptr(), F32, H * D, pages.data_ptr(), 0.125, out.data_ptr(), F32, work.data_ptr(),
+                          work.numel(), stream())
+    torch.cuda.synchronize()
+    assert (out == 7.0).all()
+    with pytest.raises(B2QError) as e:
+        engine.check_device_error()
+    assert e.value.status == EINVAL
+
+
 def test_two_prompt_calls_at_once(engine, pkg):
     """The same packed prompts on two streams at the same time, several calls each."""
     from hf_llm_b200 import paged

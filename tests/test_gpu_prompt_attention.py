@@ -192,6 +192,21 @@ def test_keys_and_queries_that_are_not_finite(engine, pkg, bad):
     assert torch.equal(out, ok)
 
 
+def test_scores_of_minus_infinity_beside_values_that_are_not_finite(engine, pkg):
+    """Key 0 scores -inf where the query's dim 5 is positive: no weight, also in
+    rows that are computed again for an infinite value behind them."""
+    q, k, v = (rand((330, h, 64), s, F16) for h, s in ((4, 1), (2, 2), (2, 3)))
+    q[:, :, 5] = q[:, :, 5].abs() + 0.1
+    k[0, :, 5] = -float("inf")
+    v[200, 0, 7] = float("inf")
+    out = run_prompt(engine, 4, 2, 64, F16, [330], [330], q, k, v, 0.1)
+    # the same without key 0, which the first query then has nothing of
+    want, bound = R.attend(q[1:200].double(), [k[1:200].double().numpy()], [v[1:200].double().numpy()], [199], 0.1, TYPES[F16],
+                           2.0 ** -19, e_prob(F16), tiny(F16, v[:200]))
+    R.check_close(out[1:200], want, bound)
+    assert torch.isinf(out[200:, :2, 7]).all()
+
+
 def test_offsets_out_of_range_are_reported(engine, pkg):
     from hf_llm_b200 import paged
     from hf_llm_b200._lib import B2QError, EINVAL

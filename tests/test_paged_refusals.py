@@ -90,7 +90,7 @@ def test_bad_gathers(calls, bad, status):
 @pytest.mark.parametrize("bad,status", [
     (dict(e=None), 1), (dict(q=None), 1), (dict(q=P + 4), 1), (dict(qs=1000), 1), (dict(pages=None), 1), (dict(pages=P + 1), 1),
     (dict(out=None), 1), (dict(out=P + 8), 1), (dict(qt=Q4_0), 6), (dict(ot=Q8_0), 6), (dict(scale=0.0), 1), (dict(scale=-1.0), 1),
-    (dict(scale=float("nan")), 1), (dict(scale=float("inf")), 1), (dict(work=None), 1), (dict(work=P + 8), 1), (dict(wb=0), 1)])
+    (dict(scale=float("nan")), 1), (dict(scale=float("inf")), 1), (dict(scale=2e30), 1), (dict(work=None), 1), (dict(work=P + 8), 1), (dict(wb=0), 1)])
 def test_bad_attention(calls, bad, status):
     assert calls["attn"](**bad) == status
 
@@ -99,7 +99,7 @@ def test_bad_attention(calls, bad, status):
     (dict(e=None), 1), (dict(n_heads=7), 1), (dict(n_kv_heads=-2), 1), (dict(head_dim=256), 6), (dict(type=F32), 6), (dict(type=Q4_0), 6),
     (dict(n_seqs=-1), 1), (dict(n_q=-1), 1), (dict(n_kv=-1), 1), (dict(max_new=-1), 1), (dict(n_seqs=70000), 1), (dict(q_start=None), 1),
     (dict(kv_start=None), 1), (dict(q=None), 1), (dict(k=None), 1), (dict(v=None), 1), (dict(out=None), 1), (dict(q=P + 2), 1),
-    (dict(ks=255), 1), (dict(vs=250), 1), (dict(qs=512), 1), (dict(scale=0.0), 1), (dict(scale=float("nan")), 1)])
+    (dict(ks=255), 1), (dict(vs=250), 1), (dict(qs=512), 1), (dict(scale=0.0), 1), (dict(scale=2e30), 1), (dict(scale=float("nan")), 1)])
 def test_bad_prompts(calls, bad, status):
     assert calls["prompt"](**bad) == status
 
