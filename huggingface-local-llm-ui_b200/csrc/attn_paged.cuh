@@ -8,18 +8,20 @@
 // 60 % of the cycles: two or three warps a scheduler is what the registers of the
 // outputs allow.  One sequence of 131072 keys, 32 heads over 8: 64 us (2.4 TB/s of
 // cache); 64 ragged sequences up to 8192 keys: 92 us; 16 sequences with five drafted
-// tokens of 64 heads over 8: 62 us; 585 keys: 12 us, launches and one join.
+// tokens of 64 heads over 8: 62 us; 585 keys: 9.3 us, most of it latency.
 //
 // Items.  The query rows (token, head) of one sequence that share a K/V head
 // are cut into blocks of 8 * NG rows; (sequence, row block, K/V head) is an
-// item, its keys are cut into tiles of 64.  All items' tiles in one line are
+// item, its keys are cut into tiles of 64.  All items' blocks of 16 keys in one line are
 // divided evenly over the CTAs and within a CTA over its warps, whatever the
 // lengths (the lengths stay on the device, so a captured call follows them).
 // A warp works alone on its tiles: a private ring of bulk copies (221 KB per
 // SM over twelve warps at D = 128), a running softmax, no barrier in the loop.  Items that end
 // inside a warp's share are written at once; the pieces of cut items are joined by
 // their CTA, and those of items cut between CTAs, through the workspace, by
-// attn_paged_join_kernel, each in order: the same bits every time.
+// attn_paged_join_kernel, each in order: the same bits every time.  Few items that
+// the page table keeps short take a cluster of CTAs each instead, which joins its
+// pieces itself (PagedArgs::whole).
 //
 // Products, on the warp-level tensor cores (mma.m16n8k16, f16 in, f32 out),
 // with the codes as exact small integers and the f16 scales applied in f32:
@@ -68,6 +70,7 @@ static_assert(2 * pg_warps(1) * pg_piece_floats(128, 1) * 4 <= pg_ring_bytes(128
 // its queries, its end and its place in the line; a warp gets at least kPgMin.
 constexpr int kPgSetup = 5, kPgMin = 1;
 constexpr int kPgMaxCtas = 256;
+constexpr int kPgMaxCluster = 8;  // (the portable size)
 
 // Who a piece of an item belongs to, and whether it holds the item's first
 // and last block.  seq < 0: no piece.
@@ -94,6 +97,7 @@ struct PagedArgs {
   int H, G;
   FastDiv dG, dKV, dPage;  // by G, by the K/V heads, by the tokens of a page
   int coarse;              // a unit of the line is 2^coarse blocks
+  int whole;               // > 0: an item is a unit, and a cluster of as many CTAs has it to itself
   const void* q;
   int q_type;
   int64_t q_stride;
@@ -141,7 +145,7 @@ __device__ __forceinline__ PgSeq pg_seq(const PagedArgs& a, int s) {
 // Units of an item, and of a sequence.  (The host picks `coarse` so that all
 // sequences at their largest stay below 2^31.)
 __device__ __forceinline__ int pg_per(const PagedArgs& a, const PgSeq& q) {
-  return ((q.nb + (1 << a.coarse) - 1) >> a.coarse) + kPgSetup;
+  return a.whole ? 1 : ((q.nb + (1 << a.coarse) - 1) >> a.coarse) + kPgSetup;
 }
 __device__ __forceinline__ int pg_units(const PagedArgs& a, const PgSeq& q) { return q.nrb * a.b.KV * pg_per(a, q); }
 
@@ -335,18 +339,19 @@ __global__ void __launch_bounds__(PgThreads<NG>::value, 1) attn_paged_kernel(con
     v0 = pg_units(a, q0);
   }
   unsigned total = pg_sum(v0);
-  if (total == kPgFull) {  // offsets that go up and down give more rows than there are: nothing is done
+  // offsets that go up and down give more rows than there are: nothing is done
+  if (total == kPgFull || (a.whole && total * a.whole > gridDim.x)) {
     if (threadIdx.x == 0) kv_batch_error();
     total = 0;
   }
-  const unsigned nc = min(gridDim.x, (total + W * kPgMin - 1) / (W * kPgMin));
+  const unsigned nc = a.whole ? total * a.whole : min(gridDim.x, (total + W * kPgMin - 1) / (W * kPgMin));
   const bool working = blockIdx.x < nc;
   if (working) {
     // the remainders go one each to the first CTAs and warps
     const unsigned per = total / nc, odd = total - per * nc;
     const unsigned c0 = per * blockIdx.x + min(blockIdx.x, odd), cn = per + (blockIdx.x < odd);
     for (int x = warp; x <= W; x += W) {  // (the first warp finds the CTA's end as well)
-      const int u = (int)(c0 + cn / W * x + min((unsigned)x, cn % W));
+      const int u = a.whole ? (int)blockIdx.x / a.whole : (int)(c0 + cn / W * x + min((unsigned)x, cn % W));
       PgAt p{};
       p.seq = a.b.n_seqs;
       if (nch > 1) {
@@ -371,6 +376,7 @@ __global__ void __launch_bounds__(PgThreads<NG>::value, 1) attn_paged_kernel(con
       } else if ((unsigned)u < total) {
         pg_place(a, 0, q0, v0, pg_scan(v0, lane), u, p);
       }
+      if (a.whole) p.blk = p.q.nb * ((int)blockIdx.x % a.whole * W + x) / (a.whole * W);
       if (lane == 0) {
         if (x < W) s_at[x] = s_ld[x] = p;
         if (x > 0) s_end[x - 1] = make_int3(p.seq, p.sub, p.blk);
@@ -927,7 +933,7 @@ __global__ void __launch_bounds__(PgThreads<NG>::value, 1) attn_paged_kernel(con
         }
       }
     } else {  // left for the join
-      const int slot = d.first ? 1 : 0;
+      const int slot = d.first && !a.whole ? 1 : 0;
       float* p = a.part + ((int64_t)blockIdx.x * 2 + slot) * pg_part_floats(D, NG);
 #pragma unroll
       for (int e = 0; e < DT / 4; ++e) *reinterpret_cast<float4*>(p + r * D + x0 + 32 * e) = v[e];
@@ -939,7 +945,53 @@ __global__ void __launch_bounds__(PgThreads<NG>::value, 1) attn_paged_kernel(con
     }
   }
   __syncthreads();
+  if (a.whole == 1) return;
   if (threadIdx.x < 2) a.desc[(int64_t)blockIdx.x * 2 + threadIdx.x] = s_out[threadIdx.x];
+  if (a.whole == 0) return;
+  // ---- the cluster's pieces of its item, in order, a share of the row's dims to each CTA ----
+  asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
+  if (!working) return;
+  const int cs = a.whole, rank = (int)blockIdx.x % cs, c0 = (int)blockIdx.x - rank;
+  const PgAt at = s_at[0];  // (any place of the item: the plan's, or where its warp stopped)
+  for (int x = rank * (32 * W) + (int)threadIdx.x; x < R * (D / 4); x += cs * (32 * W)) {
+    const int r = x / (D / 4), d4 = x % (D / 4) * 4;
+    float2 rs[kPgMaxCluster];
+    float4 y[kPgMaxCluster];
+    int has[kPgMaxCluster];
+#pragma unroll
+    for (int k = 0; k < kPgMaxCluster; ++k) {  // (all on their way at once; a CTA without a piece left anything)
+      const int c = c0 + min(k, cs - 1);
+      const float* p = a.part + (int64_t)c * 2 * pg_part_floats(D, NG);
+      has[k] = k < cs ? __ldcg(&a.desc[(int64_t)c * 2].seq) : -1;
+      rs[k] = __ldcg(reinterpret_cast<const float2*>(p + R * D + 2 * r));
+      y[k] = __ldcg(reinterpret_cast<const float4*>(p + r * D + d4));
+    }
+    float rf = -INFINITY, l = 0.0f;
+    bool any = false;
+#pragma unroll
+    for (int k = 0; k < kPgMaxCluster; ++k)
+      if (has[k] >= 0) {
+        any = true;
+        rf = fmaxf(rf, rs[k].x);
+      }
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int k = 0; k < kPgMaxCluster; ++k)
+      if (has[k] >= 0) {
+        const float w = pg_weight(rs[k].x, rf);
+        l = fmaf(w, rs[k].y, l);
+        v.x = fmaf(w, y[k].x, v.x);
+        v.y = fmaf(w, y[k].y, v.y);
+        v.z = fmaf(w, y[k].z, v.z);
+        v.w = fmaf(w, y[k].w, v.w);
+      }
+    const int rb = fdiv(at.sub, a.dKV), h = at.sub - rb * a.b.KV;
+    if (any && rb * R + r < at.q.rows) {
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      const float f[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
+      pg_store4(a, pg_out_row(a, at.q.qa, rb * R + r, h, D) + d4, f);
+    }
+  }
 }
 
 // Items cut between CTAs: CTA c joins the item that c begins and does not

@@ -138,10 +138,18 @@ static cudaError_t launch_paged(const PagedArgs& a, int ctas, int device, cudaSt
   static std::atomic<uint64_t> done{0};
   cudaError_t err = allow_smem(attn_paged_kernel<D, NG, QSPLIT, PSPLIT>, pg_ring_bytes(D, NG), device, done);
   if (err != cudaSuccess) return err;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[1], both[2];
   cudaLaunchConfig_t cfg = dependent_launch((unsigned)ctas, pg_warps(NG) * 32, pg_ring_bytes(D, NG), st, attr);
+  if (a.whole > 1) {
+    both[0] = attr[0];
+    both[1].id = cudaLaunchAttributeClusterDimension;
+    both[1].val.clusterDim.x = (unsigned)a.whole;
+    both[1].val.clusterDim.y = both[1].val.clusterDim.z = 1;
+    cfg.attrs = both;
+    cfg.numAttrs = 2;
+  }
   err = cudaLaunchKernelEx(&cfg, attn_paged_kernel<D, NG, QSPLIT, PSPLIT>, a);
-  if (err != cudaSuccess) return err;
+  if (err != cudaSuccess || a.whole) return err;
   cfg.blockDim = dim3(kPgJoinThreads);
   cfg.dynamicSmemBytes = 0;
   return cudaLaunchKernelEx(&cfg, attn_paged_join_kernel<D, NG>, a);
@@ -352,13 +360,31 @@ b2q_status b2q_attn_paged_dev(b2q_engine* e, const b2q_kv_config* cfg, const b2q
   const bool wide = qt != kElF32 && (int64_t)batch->max_new * a.G > 8;
   // the probabilities' second part where the output shows it
   const bool split = ot == kElF32;
+  // Few items that the page table keeps short: a cluster of CTAs to each, the more
+  // the better down to half a block of keys a warp, and no second launch.  Device
+  // times so / by the line, 8 K/V heads: one sequence of 100 tokens 8.1 / 8.9 us, 585
+  // 9.3 / 11.8, 2048 11.5 / 13.3; four of 1024 11.7 / 13.6, of 2048 (2.7 blocks a
+  // warp) 16.1 / 14.6: the line leaves no SM without work.
+  // (sequences with rows: k at most, so row blocks: (rows + k (R - 1)) / R at most)
+  const int warps = pg_warps(wide ? 2 : 1), R = pg_rows(wide ? 2 : 1);
+  const int64_t k = std::min(a.b.n_seqs, a.b.n_tokens);
+  const int64_t few = std::min(((int64_t)a.b.n_tokens * a.G + k * (R - 1)) / R, (int64_t)a.b.n_tokens * ((a.G + R - 1) / R)) * a.b.KV;
+  // (the larger a cluster the fewer SMs a GPU full of them reaches: 16 of eight CTAs took
+  // two rounds, two sequences of 585 tokens 16.7 us; in clusters of four 10.5)
+  int cluster = 1;
+  if (blocks > warps)
+    while (cluster < kPgMaxCluster && 2 * cluster * few <= (cluster == 1 ? ctas : cluster == 2 ? ctas * 7 / 8 : ctas * 2 / 3) &&
+           2 * blocks > cluster * warps)
+      cluster *= 2;
+  a.whole = cluster * few <= ctas && blocks <= 2 * cluster * warps ? cluster : 0;
+  const int grid = a.whole ? (int)(few * cluster) : ctas;
   cudaError_t err = cudaSuccess;
   by_dim(D, [&](auto d) {
-    if (wide) err = split ? launch_paged<d(), 2, false, true>(a, ctas, e->device, st) : launch_paged<d(), 2, false, false>(a, ctas, e->device, st);
-    else if (qt == kElF32) err = split ? launch_paged<d(), 1, true, true>(a, ctas, e->device, st) : launch_paged<d(), 1, true, false>(a, ctas, e->device, st);
-    else err = split ? launch_paged<d(), 1, false, true>(a, ctas, e->device, st) : launch_paged<d(), 1, false, false>(a, ctas, e->device, st);
+    if (wide) err = split ? launch_paged<d(), 2, false, true>(a, grid, e->device, st) : launch_paged<d(), 2, false, false>(a, grid, e->device, st);
+    else if (qt == kElF32) err = split ? launch_paged<d(), 1, true, true>(a, grid, e->device, st) : launch_paged<d(), 1, true, false>(a, grid, e->device, st);
+    else err = split ? launch_paged<d(), 1, false, true>(a, grid, e->device, st) : launch_paged<d(), 1, false, false>(a, grid, e->device, st);
   });
-  launch_counted(e, 2);
+  launch_counted(e, a.whole ? 1 : 2);
   return err == cudaSuccess ? B2Q_OK : cuda_error(err, what);
 }
 

@@ -333,7 +333,8 @@ typedef struct {
   int kv_type;     /* B2Q_Q4_0: blocks of 32 values, 4-bit codes and one f16 scale */
   int page_tokens; /* tokens of a page: a multiple of 16, at most 4096 */
   int n_pages;     /* pages of the pool */
-  int max_pages;   /* row length of the page table; max_pages * page_tokens <= 2^30 */
+  int max_pages;   /* row length of the page table; max_pages * page_tokens <= 2^30 (what it has
+                    * room for bounds the lengths: few short sequences take less time with a short one) */
 } b2q_kv_config;
 
 /* The tokens of one call.  Sequence s has the packed rows q_start[s] ..

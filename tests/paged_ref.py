@@ -79,6 +79,9 @@ def block_bytes(kc, ks, vc, vs) -> np.ndarray:
     return out
 
 
+MORE_PAGES = 0  # unused entries of every row of a pool's page table
+
+
 class Pool:
     """A pool of pages with the batch arrays of `lens` cached and `news` new
     tokens a sequence.  Every byte that no token's place covers is 0xff (NaN
@@ -89,7 +92,7 @@ class Pool:
         self.H, self.KV, self.D, self.P, self.lens, self.news = heads, kv_heads, dim, page, list(lens), list(news)
         rng = np.random.default_rng(seed)
         need = [(l + page - 1) // page for l in lens]
-        self.max_pages = max_pages or max(1, max(need))
+        self.max_pages = max_pages or max(1, max(need)) + MORE_PAGES
         self.n_pages = sum(need) + spare
         perm = rng.permutation(self.n_pages)
         table = np.full((len(lens), self.max_pages), -7, np.int32)  # unused entries are no pages

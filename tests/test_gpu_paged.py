@@ -14,6 +14,16 @@ from paged_ref import BF16, F16, F32, Pool, TYPES
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(autouse=True, params=[0, 4000], ids=["short table", "long table"])
+def table(request):
+    """What a page table has room for decides how few sequences are divided among
+    the CTAs: an item to a cluster, or all of them as one line."""
+    R.MORE_PAGES = request.param
+    yield
+    R.MORE_PAGES = 0
+
+
+
 def stream():
     return torch.cuda.current_stream().cuda_stream or 1
 

@@ -10,7 +10,7 @@ import torch
 
 import paged_ref as R
 from paged_ref import BF16, F16, F32, Pool, TYPES
-from test_gpu_paged import E_SCORE, check_paged, e_prob, expected_pages, rand, run_append, run_paged, stream, tiny
+from test_gpu_paged import E_SCORE, check_paged, e_prob, expected_pages, rand, run_append, run_paged, stream, table, tiny  # noqa: F401
 from test_gpu_prompt_attention import check as check_prompt
 from test_gpu_prompt_attention import e_prob as e_prob_prompt, tiny as tiny_prompt
 
@@ -37,8 +37,8 @@ class Layer:
             self.w.append((w, engine.try_upload_weight(raw.reshape(-1), Q8_0, n, E)))
         mp = (room + page - 1) // page
         perm = rng.permutation(n_seqs * mp).astype(np.int32).reshape(n_seqs, mp)
-        self.cfg = paged.kv_config(H, KV, D, R.Q4_0, page, n_seqs * mp, mp)
-        self.table = torch.from_numpy(perm).cuda()
+        self.cfg = paged.kv_config(H, KV, D, R.Q4_0, page, n_seqs * mp, mp + R.MORE_PAGES)
+        self.table = torch.from_numpy(np.pad(perm, ((0, 0), (0, R.MORE_PAGES)), constant_values=-7)).cuda()
         self.pages = torch.full((n_seqs * mp * paged.page_bytes(self.cfg),), 0xff, dtype=torch.uint8, device="cuda")
         self.cos, self.sin = R.rope_tables(room, D)
         self.dev_tables = torch.from_numpy(self.cos).cuda(), torch.from_numpy(self.sin).cuda()
