@@ -5,7 +5,7 @@
 // The cache is read once, 18 * D bytes for 16 keys and values of a head, and
 // that stream is the floor.  What bounds the kernel is the instructions beside it
 // (some 530 a warp for 16 keys and 16 rows, half of them unpacking), issued on 43 to
-// 60 % of the cycles: two or three warps a scheduler is what the registers of the
+// 52 % of the cycles: two or three warps a scheduler is what the registers of the
 // outputs allow.  One sequence of 131072 keys, 32 heads over 8: 64 us (2.4 TB/s of
 // cache); 64 ragged sequences up to 8192 keys: 92 us; 16 sequences with five drafted
 // tokens of 64 heads over 8: 62 us; 585 keys: 9.3 us, most of it latency.
