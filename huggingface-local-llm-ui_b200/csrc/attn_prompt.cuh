@@ -22,12 +22,12 @@
 // What bounds it: the matrix unit (16 instructions of 64 cycles for each row tile
 // and 128 keys, more like 90 with the softmax's TMEM traffic beside them) and, close
 // behind, a softmax of 1640 cycles that has to be done when the other row tile's
-// products are.  Measured at 8192 tokens of 64 heads, 893 us (1.23 PFLOP/s): keeping
+// products are.  Measured at 8192 tokens of 64 heads, 900 us (1.22 PFLOP/s): keeping
 // the issuing warp converged, with one elected thread, 981 -> 910 us (a branch on the
 // lane moved every descriptor between register files); the next item's geometry
 // under the last product and stores of 64 consecutive bytes, 910 -> 893 (16 ragged
 // prompts 172 -> 157).  That is a burst; where the power cap holds the clock at 1.6
-// to 1.7 GHz it takes 1046.  16 tokens behind 2048, 32 heads over 8: 23 us in halves,
+// to 1.7 GHz it takes 1050.  16 tokens behind 2048, 32 heads over 8: 23 us in halves,
 // 32.5 without (512 tokens behind 2048: 29 and 39).  Tried on the 984 us form: a
 // quarter of the exponentials by a polynomial on the FMA units, 1040; two threads to
 // a row, 1027; key tiles of 64 with two score buffers, 1270 (a score product of 64
