@@ -32,9 +32,10 @@
 //      where the output is f32), one B for each 32 dims.
 // (Codes left where they lie, as f16 subnormals, would halve the unpacking, but
 // the matrix unit aligns products by their nominal exponents: 2^-17 is lost.)
-// The softmax reference is shifted by the largest value scale seen and follows
-// the maximum in steps of 2^8, so that p_j * scale_j lies between 2^6 and 2^15 where
-// it is largest: f16's subnormals are far below, and outputs are seldom rescaled.
+// A row's softmax reference follows the largest p_j * scale_j of the keys that the row
+// sees (the largest scale of a key's blocks of dims) in steps of 2^8, so that it lies
+// between 2^7 and 2^15: a product keeps its bits down to 2^-32 of that one (f16's
+// smallest step is 2^-24), and outputs are seldom rescaled.
 #pragma once
 
 #include <type_traits>
@@ -214,6 +215,12 @@ __device__ __forceinline__ int pg_keys(const PagedArgs& a, const PgAt& p) {
 __device__ __forceinline__ float pg_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float pg_log2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -480,7 +487,6 @@ __global__ void __launch_bounds__(PgThreads<NG>::value, 1) attn_paged_kernel(con
   float o[NG][D / 16][4];
   float mx[NG], ref[NG], sum[NG], fac[NG];
   int lim[NG];
-  int ev = -24;   // exponent of the largest value scale so far
   int keys = 0, min_lim = 0;
   int at_blk = 0, at_end = 0;
   auto begin = [&]() {
@@ -528,7 +534,6 @@ __global__ void __launch_bounds__(PgThreads<NG>::value, 1) attn_paged_kernel(con
       for (int m = 0; m < D / 16; ++m) o[n][m][0] = o[n][m][1] = o[n][m][2] = o[n][m][3] = 0.0f;
     }
     min_lim = min(at.q.base + fdiv(rb * R, a.dG), keys - 1);
-    ev = -24;
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -551,34 +556,30 @@ __global__ void __launch_bounds__(PgThreads<NG>::value, 1) attn_paged_kernel(con
   // half of the time) ----
   auto tile = [&](const uint8_t* tb, uint32_t vm) {
     const int key0 = at_blk * kKvBlk;
-    // largest value scale of the tile (magnitudes of f16 order like their bits)
+    // log2 of the largest value scale of tokens 2 lane and 2 lane + 1 of the tile.  (The
+    // larger of a number and NaN is the number; what is not finite, or zero, counts as
+    // the nearest scale that is, and shows in the products.)
+    float lg[2];
     {
-      constexpr int TL = 8 / NB;       // tokens of a 16-byte piece of scales
-      constexpr int LB = kKvBlk / TL;  // pieces of a block
-      const int blk = lane / LB, tok = (lane % LB) * TL;
-      __half2 m = __float2half2_rn(0.0f);
-      if (lane < kPgBlks * LB && ((vm >> blk) & 1)) {
-        uint4 x = *reinterpret_cast<const uint4*>(tb + blk * BB + 17 * D + tok * NB * 2);
-        const int left = keys - key0 - blk * kKvBlk - tok;  // tokens of the piece that are keys
-        if (left < TL) {
-          if (NB == 4) {
-            if (left <= 0) x.x = x.y = 0u;
-            if (left <= 1) x.z = x.w = 0u;
-          } else {
-            if (left <= 0) x.x = 0u;
-            if (left <= 1) x.y = 0u;
-            if (left <= 2) x.z = 0u;
-            if (left <= 3) x.w = 0u;
-          }
+      const int blk = lane >> 3;
+      uint32_t m[2] = {0u, 0u};
+      if ((vm >> blk) & 1) {
+        const uint8_t* sp = tb + blk * BB + 17 * D + (lane & 7) * 2 * NB * 2;
+        if (NB == 4) {
+          const uint4 x = *reinterpret_cast<const uint4*>(sp);
+          m[0] = h2_u32(__hmax2(__habs2(u32_h2(x.x)), __habs2(u32_h2(x.y))));
+          m[1] = h2_u32(__hmax2(__habs2(u32_h2(x.z)), __habs2(u32_h2(x.w))));
+        } else {
+          const uint2 x = *reinterpret_cast<const uint2*>(sp);
+          m[0] = h2_u32(__habs2(u32_h2(x.x)));
+          m[1] = h2_u32(__habs2(u32_h2(x.y)));
         }
-        // (the larger of a number and NaN is the number; infinities show anyway)
-        m = __hmax2(__hmax2(__habs2(u32_h2(x.x)), __habs2(u32_h2(x.y))), __hmax2(__habs2(u32_h2(x.z)), __habs2(u32_h2(x.w))));
       }
-      const uint32_t u = h2_u32(m), v0 = u & 0x7fffu, v1 = u >> 16 & 0x7fffu;
-      uint32_t big = max(v0 < 0x7c00u ? v0 : 0u, v1 < 0x7c00u ? v1 : 0u);
-      big = __reduce_max_sync(B2Q_FULL, big);
-      const int e = big >= 0x400u ? (int)(big >> 10) - 15 : big ? 7 - __clz(big) : -24;
-      ev = max(ev, e);  // (subnormal: the leading bit's place, 2^-24 upward)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float2 f = __half22float2(u32_h2(m[e]));
+        lg[e] = pg_log2(fminf(fmaxf(fmaxf(f.x, f.y), 0x1p-24f), 65504.0f));
+      }
     }
     float ta[NG][D / 16][4];
     if (PSPLIT) {
@@ -650,23 +651,29 @@ __global__ void __launch_bounds__(PgThreads<NG>::value, 1) attn_paged_kernel(con
               if (k > lim[n] || k >= keys) s[n][x][e] = -INFINITY;
             }
       }
-      // softmax: the reference moves when a row's maximum, or the largest value
-      // scale, has outgrown it by 2^8 (p * scale then stays below 2^15)
+      // softmax: the reference moves when a product of a probability and a value scale
+      // that the row sees has outgrown it by 2^15 (the largest product since it last
+      // moved is 2^7 or above)
+      float sl[2][2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) sl[x][e] = __shfl_sync(B2Q_FULL, lg[e], 8 * j + 4 * x + t);
       bool move = false;
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
-        float tm = fmaxf(fmaxf(s[n][0][0], s[n][0][1]), fmaxf(s[n][1][0], s[n][1][1]));
+        float tm = fmaxf(fmaxf(fmaf(s[n][0][0], fac[n], sl[0][0]), fmaf(s[n][0][1], fac[n], sl[0][1])),
+                         fmaxf(fmaf(s[n][1][0], fac[n], sl[1][0]), fmaf(s[n][1][1], fac[n], sl[1][1])));
         tm = fmaxf(tm, __shfl_xor_sync(B2Q_FULL, tm, 1));
-        tm = fmaxf(tm, __shfl_xor_sync(B2Q_FULL, tm, 2));
-        mx[n] = fmaxf(mx[n], tm * fac[n]);
-        move = move || mx[n] + (float)(ev - 14) > ref[n];
+        mx[n] = fmaxf(mx[n], fmaxf(tm, __shfl_xor_sync(B2Q_FULL, tm, 2)));
+        move = move || mx[n] - 15.0f > ref[n];
       }
       if (__any_sync(B2Q_FULL, move)) {
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
           float cr = 1.0f;
-          if (mx[n] + (float)(ev - 14) > ref[n]) {
-            const float nref = mx[n] + (float)(ev - 6);
+          if (mx[n] - 15.0f > ref[n]) {
+            const float nref = mx[n] - 7.0f;
             cr = pg_weight(ref[n], nref);
             ref[n] = nref;
           }

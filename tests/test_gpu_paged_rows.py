@@ -1,0 +1,100 @@
+"""Rows of the paged attention that one call treats apart: the precision of a row
+hangs on what that row sees."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import paged_ref as R
+from paged_ref import BF16, F16, F32, TYPES, Pool
+from test_gpu_paged import E_SCORE, e_prob, rand, run_paged, table  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def scale_tokens(pool, s, positions, factor, keys=False):
+    """Multiplies the value (or key) scales of positions of sequence s by a power of two."""
+    at = (8 if keys else 17) * pool.D
+    for p in positions:
+        blk = pool.pages[pool.table[s, p // pool.P], :, p % pool.P // 16]
+        sc = blk[:, at:at + pool.D].copy().view(np.float16).reshape(pool.KV, 16, -1)
+        new = (sc[:, p % 16].astype(np.float32) * factor).astype(np.float16)
+        assert (new.astype(np.float32) == sc[:, p % 16].astype(np.float32) * factor).all()
+        sc[:, p % 16] = new
+        blk[:, at:at + pool.D] = sc.reshape(pool.KV, -1).view(np.uint8)
+
+
+def value_scales(pool, s):
+    """[len, KV]: the largest value scale of each token."""
+    out = np.zeros((pool.lens[s], pool.KV))
+    for p in range(pool.lens[s]):
+        blk = pool.pages[pool.table[s, p // pool.P], :, p % pool.P // 16]
+        sc = blk[:, 17 * pool.D:].copy().view(np.float16).reshape(pool.KV, 16, -1)
+        out[p] = np.abs(sc[:, p % 16].astype(np.float64)).max(-1)
+    return out
+
+
+def check_rows(out, pool, ks, vs, q, scale, q_type, out_type):
+    """Each row against f64 by itself.  A probability times its value's scale enters as
+    f16, one part or two, and the largest such product that the row has is 2^7 or above: a
+    term is off by 2^-25 (half of f16's smallest step) beside its relative error, so by 2^-32
+    of that product, times |code - 8| <= 8.  (1.02: the kernel's own probabilities.)"""
+    G, a = pool.H // pool.KV, 0
+    for s, n in enumerate(pool.news):
+        l, top = pool.lens[s], value_scales(pool, s)
+        for i in range(n):
+            see = l - n + i + 1
+            x = q[a + i].double()
+            for h in range(pool.H):
+                w = torch.from_numpy(ks[s][:see, h // G]) @ x[h] * scale
+                m = float((torch.softmax(w, 0) * torch.from_numpy(top[:see, h // G])).max())
+                want, bound = R.attend(x[None, h:h + 1], [ks[s][:see, h // G:h // G + 1]], [vs[s][:see, h // G:h // G + 1]], [1], scale,
+                                       TYPES[out_type], E_SCORE, e_prob(out_type), 1.02 * 2.0 ** -29 * m)
+                R.check_close(out[a + i:a + i + 1, h:h + 1], want, bound)
+        a += n
+
+
+@pytest.mark.parametrize("heads,kv,dim,lens,news,q_type,out_type", [
+    (8, 2, 128, [300, 40], [5, 3], F32, F32),
+    (16, 2, 64, [70, 33], [4, 2], F16, F32),     # 16 rows to an item
+    (8, 1, 128, [130], [3], BF16, BF16),
+    (4, 4, 64, [17, 64], [2, 5], F32, F16),
+])
+def test_a_row_keeps_its_bits_beside_values_it_does_not_see(engine, pkg, heads, kv, dim, lens, news, q_type, out_type):
+    """The last new token's values are 2^27 times the others'."""
+    pool = Pool(heads, kv, dim, 16, lens, news, seed=2)
+    ks, vs = pool.fill()
+    for s, l in enumerate(lens):
+        scale_tokens(pool, s, range(l - 1), 2.0 ** -10)
+        scale_tokens(pool, s, [l - 1], 2.0 ** 17)
+        vs[s][:l - 1] *= 2.0 ** -10
+        vs[s][l - 1] *= 2.0 ** 17
+    q = rand((pool.rows, heads, dim), 5, q_type)
+    out = run_paged(engine, pool.upload(), q, q_type, out_type, dim ** -0.5)
+    check_rows(out, pool, ks, vs, q, dim ** -0.5, q_type, out_type)
+    engine.check_device_error()
+
+
+@pytest.mark.parametrize("q_type,out_type", [(F32, F32), (F16, F16)])
+@pytest.mark.parametrize("at", [0, 7, 100, 298])
+def test_large_values_without_weight(engine, pkg, q_type, out_type, at):
+    """One token with values 2^27 times the others' and a probability below 2^-50."""
+    pool = Pool(8, 2, 128, 16, [300], [1], seed=2)
+    ks, vs = pool.fill()
+    scale_tokens(pool, 0, [p for p in range(300) if p != at], 2.0 ** -10)
+    scale_tokens(pool, 0, [at], 2.0 ** 17)
+    scale_tokens(pool, 0, [at], 8.0, keys=True)
+    f = np.where(np.arange(300) == at, 2.0 ** 17, 2.0 ** -10)[:, None, None]
+    vs[0] *= f
+    ks[0][at] *= 8.0
+    # queries that point away from that token's key
+    q = rand((1, 8, 128), 5).double()
+    for h in range(8):
+        k = torch.from_numpy(ks[0][at, h // 4])
+        q[0, h] -= 6.0 * k / k.norm() + (q[0, h] @ k) * k / (k @ k)
+    q = q.to(TYPES[q_type])
+    w = torch.einsum("hd,hd->h", q[0].double(), torch.from_numpy(ks[0][at]).repeat_interleave(4, 0)) * 128 ** -0.5
+    assert (w < -36).all()  # e^-36 < 2^-51
+    out = run_paged(engine, pool.upload(), q, q_type, out_type, 128 ** -0.5)
+    check_rows(out, pool, ks, vs, q, 128 ** -0.5, q_type, out_type)
