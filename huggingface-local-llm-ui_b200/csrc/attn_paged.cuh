@@ -114,7 +114,7 @@ struct PagedArgs {
 // The part of a sequence's geometry that the plan needs.
 struct PgSeq {
   int qa, n;      // first row, rows of this call
-  int base, len;  // position of the first row (may be negative), cached tokens
+  int base, len;  // position of the first row (may be negative), cached tokens that the table has room for
   int rows;       // n * G
   int nb, nrb;    // blocks of an item (16 keys), row blocks
 };
@@ -128,7 +128,7 @@ __host__ __device__ inline PgSeq pg_seq_of(int qa, int qe, int len, int n_tokens
   s.n = ok ? (qe < n_tokens ? qe : n_tokens) - qa : 0;
   if (s.n < 0) s.n = 0;
   s.len = len < 0 ? 0 : len > cap ? cap : len;
-  s.base = s.len - n_all;
+  s.base = (len < 0 ? 0 : len) - n_all;  // (below 0 cached tokens no row has a position, as with 0)
   s.rows = s.n * G;
   s.nb = s.len > kKvBlk ? (s.len + kKvBlk - 1) / kKvBlk : 1;  // (one for none: its rows become zeros)
   s.nrb = (s.rows + R - 1) / R;
@@ -272,6 +272,11 @@ __device__ __forceinline__ void pg_store4(const PagedArgs& a, int64_t i, const f
   if (a.out_type == kElF32) st4(reinterpret_cast<float*>(a.out) + i, v);
   else if (a.out_type == kElF16) st4(reinterpret_cast<__half*>(a.out) + i, v);
   else st4(reinterpret_cast<__nv_bfloat16*>(a.out) + i, v);
+}
+// Whether row r of the sequence is one, and has a position: one of a length beyond the
+// page table, or of fewer cached tokens than new ones, is left as it is.
+__device__ __forceinline__ bool pg_row_live(const PagedArgs& a, const PgSeq& q, int r) {
+  return r < q.rows && (unsigned)(q.base + fdiv(r, a.dG)) < (unsigned)(a.b.max_pages * a.b.page_tokens);
 }
 // Index of row r (of a sequence from row qa on) of K/V head h in out (and, with
 // the token stride, in q).
@@ -852,7 +857,7 @@ __global__ void __launch_bounds__(PgThreads<NG>::value, 1) attn_paged_kernel(con
           const float l = __shfl_sync(B2Q_FULL, sum[n], 8 * t + 4 * e);
           const float inv = l == 0.0f ? 0.0f : 1.0f / l;
           const int r = rb * R + 8 * n + 2 * t + e;
-          if (r < at.q.rows) {
+          if (pg_row_live(a, at.q, r)) {
             const int64_t i0 = pg_out_row(a, at.q.qa, r, h, D);
 #pragma unroll
             for (int m = 0; m < D / 16; ++m) {
@@ -930,7 +935,7 @@ __global__ void __launch_bounds__(PgThreads<NG>::value, 1) attn_paged_kernel(con
     if (d.first && whole_last) {
       const PgSeq q = pg_seq<NG>(a, d.seq);
       const int rb = fdiv(d.sub, a.dKV), h = d.sub - rb * a.b.KV;
-      if (rb * R + r < q.rows) {
+      if (pg_row_live(a, q, rb * R + r)) {
         const int64_t i0 = pg_out_row(a, q.qa, rb * R + r, h, D) + x0;
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
@@ -993,7 +998,7 @@ __global__ void __launch_bounds__(PgThreads<NG>::value, 1) attn_paged_kernel(con
         v.w = fmaf(w, y[k].w, v.w);
       }
     const int rb = fdiv(at.sub, a.dKV), h = at.sub - rb * a.b.KV;
-    if (any && rb * R + r < at.q.rows) {
+    if (any && pg_row_live(a, at.q, rb * R + r)) {
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       const float f[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
       pg_store4(a, pg_out_row(a, at.q.qa, rb * R + r, h, D) + d4, f);
@@ -1064,7 +1069,7 @@ __global__ void __launch_bounds__(kPgJoinThreads) attn_paged_join_kernel(const _
   }
   const PgSeq q = pg_seq<NG>(a, d.seq);
   const int rb = fdiv(d.sub, a.dKV), h = d.sub - rb * a.b.KV;
-  if (rb * R + r >= q.rows) return;
+  if (!pg_row_live(a, q, rb * R + r)) return;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   const float f[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
   pg_store4(a, pg_out_row(a, q.qa, rb * R + r, h, D) + d4, f);

@@ -393,7 +393,9 @@ b2q_status b2q_kv_gather_dev(b2q_engine* eng, const b2q_kv_config* cfg, const b2
  * keys and values are appended already) over the cache: query head h reads
  * K/V head h / (n_heads / n_kv_heads),
  * out = sum_j p_j v_j / sum_j p_j, p_j = exp(scale * q.k_j), over the
- * positions j up to the token's own.  A token without keys gives zeros.
+ * positions j up to the token's own.  A token none of whose keys has a valid
+ * page gives zeros; one without a valid position (kv_len beyond the table's
+ * room, or below the sequence's new tokens) is left as it is.
  * Sums and the softmax in f32; f32 queries are carried as two f16 parts
  * (~2^-22), and so is a probability times its value's scale where out is f32;
  * for 16-bit outputs that product is rounded once, to f16.  Beside that such a

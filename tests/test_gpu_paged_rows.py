@@ -1,5 +1,5 @@
 """Rows of the paged attention that one call treats apart: the precision of a row
-hangs on what that row sees."""
+hangs on what that row sees, and rows without a valid position are left as they are."""
 from __future__ import annotations
 
 import numpy as np
@@ -98,3 +98,40 @@ def test_large_values_without_weight(engine, pkg, q_type, out_type, at):
     assert (w < -36).all()  # e^-36 < 2^-51
     out = run_paged(engine, pool.upload(), q, q_type, out_type, 128 ** -0.5)
     check_rows(out, pool, ks, vs, q, 128 ** -0.5, q_type, out_type)
+
+
+def rows_left(engine, pool, ks, vs, q, q_type, claimed, cap, scale=0.125):
+    """Runs with kv_len = claimed: rows with a position in [0, cap) attend the keys that the
+    table has, the others keep what they held."""
+    from hf_llm_b200._lib import B2QError, EINVAL
+    n, real = pool.news[0], pool.lens[0]
+    pool.dev["kv_len"][0] = claimed
+    out = run_paged(engine, pool, q, q_type, q_type, scale)
+    with pytest.raises(B2QError) as e:
+        engine.check_device_error()
+    assert e.value.status == EINVAL
+    for i in range(n):
+        pos = claimed - n + i
+        if 0 <= pos < cap:
+            see = min(pos + 1, real)
+            want, bound = R.attend(q[i:i + 1].double(), [ks[0][:see]], [vs[0][:see]], [1], scale, TYPES[q_type], E_SCORE, e_prob(q_type),
+                                   2.0 ** -28 * pool.largest_scale())
+            R.check_close(out[i:i + 1], want, bound)
+        else:
+            assert (out[i] == 7.0).all(), (i, pos)
+    want, bound = R.attend(q[n:pool.T].double(), ks[1:], vs[1:], pool.news[1:], scale, TYPES[q_type], E_SCORE, e_prob(q_type),
+                           2.0 ** -28 * pool.largest_scale())
+    R.check_close(out[n:pool.T], want, bound)
+
+
+@pytest.mark.parametrize("q_type", [F32, F16])
+@pytest.mark.parametrize("pages,page", [(4, 16), (16, 256)])  # a cluster an item; one line, joined by a second launch
+def test_rows_without_a_position_are_left_as_they_are(engine, pkg, q_type, pages, page):
+    cap = pages * page
+    pool = Pool(8, 1, 64, page, [cap, 20], [4, 2], max_pages=pages)
+    ks, vs = pool.fill()
+    pool.upload()
+    q = rand((pool.rows, 8, 64), 5, q_type)
+    # the sequence's keys are those of the table, whatever kv_len claims
+    for claimed in (cap + 1, cap + 3, cap + 4, cap + 100, 2 ** 31 - 1, 3, 1, 0, -1, -2 ** 31):
+        rows_left(engine, pool, ks, vs, q, q_type, claimed, cap)
