@@ -821,7 +821,7 @@ __global__ void __launch_bounds__(PgThreads<NG>::value, 1) attn_paged_kernel(con
     if (!__all_sync(B2Q_FULL, mbar_wait_bounded(&bars[warp][st], phase))) {
       // a wait gave up (the error word is set): first the copies in flight
       for (int k = 0; k < in_flight; ++k) {
-        mbar_wait_bounded(&bars[warp][st], phase);
+        mbar_drain(&bars[warp][st], phase);
         if (++st == S) {
           st = 0;
           phase ^= 1;

@@ -544,7 +544,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
       if (lane == 0) {
         const uint32_t qbytes = (uint32_t)(a.tpt * a.gp * 128 * NC);
         uint32_t ph = 0, land = 0, q_ph = 0;        // phases: of the ring, bits per stage, bits per row tile
-        uint32_t used = 0, looks = 0;               // for a failure: stages loaded, by which barrier
+        uint32_t used = 0, looks = 0;               // for the end: stages loaded, by which barrier
         int st = 0, qn = 0;
         bool ok = true;
         for (int round = 0; ok && round < rounds; ++round) {
@@ -587,15 +587,14 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
             if (x == 0 && it.nq == 2) ok = load_q(1);
           }
         }
-        if (!ok) {  // copies in flight land before the CTA may end
-          *s_fail = 1;
-          for (int i = 0; i < 2; ++i)
-            if (qn >> i & 1) mbar_wait_bounded(&q_full[i], ((q_ph >> i) & 1) ^ 1);
-          for (int x = 0; x < NS; ++x) {
-            if (!(used >> x & 1)) continue;
-            if (looks >> x & 1) mbar_wait_bounded(&v_land[x], ((land >> x) & 1) ^ 1);
-            else mbar_wait_bounded(&full[x], x < st ? ph : ph ^ 1);
-          }
+        if (!ok) *s_fail = 1;
+        // copies in flight land before the CTA may end, whichever warp gave up
+        for (int i = 0; i < 2; ++i)
+          if (qn >> i & 1) mbar_drain(&q_full[i], ((q_ph >> i) & 1) ^ 1);
+        for (int x = 0; x < NS; ++x) {
+          if (!(used >> x & 1)) continue;
+          if (looks >> x & 1) mbar_drain(&v_land[x], ((land >> x) & 1) ^ 1);
+          else mbar_drain(&full[x], x < st ? ph : ph ^ 1);
         }
       }
     } else if (warp == 9) {
@@ -684,11 +683,11 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
           }
         }
       }
-      if (!ok) {  // whatever was issued completes before the TMEM is freed
-        *s_fail = 1;
-        if (pr_elect()) pr_commit(&done);
-        mbar_wait_bounded(&done, 0);
-      }
+      if (!ok) *s_fail = 1;
+      // whatever was issued completes before the TMEM is freed, whichever warp gave up
+      __syncwarp();
+      if (pr_elect()) pr_commit(&done);
+      mbar_drain(&done, 0);
     } else {
       // ---- value tiles that some row sees only in part ----
       const int w = threadIdx.x - 320;  // 0..63: rows w and w + 64

@@ -209,6 +209,16 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
   return true;
 }
 
+// Wait for what is still in flight on `bar` before its memory is given up,
+// after a wait gave up.  Bounded by the default limit whatever the host set (a
+// copy or a product outlasts a lowered one), and silent: the error word is
+// raised already.
+__device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
+  const long long t0 = clock64();
+  while (!mbar_try_wait(bar, parity) && clock64() - t0 <= kSpinLimitCycles) {
+  }
+}
+
 // Global -> shared bulk copy of `bytes` (multiple of 16, both addresses
 // 16-byte aligned), completing on `bar` as transaction bytes.
 __device__ __forceinline__ void bulk_g2s(void* dst, const void* src, uint32_t bytes,

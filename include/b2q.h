@@ -561,8 +561,10 @@ b2q_status b2q_debug_check_site(b2q_engine* eng, int* site);
 /* Upper bound of every device-side wait of this engine's GPU (mbarriers,
  * grid and all-rank barriers, tagged hand-offs), in SM clock cycles;
  * cycles <= 0 restores the default 4e9 (~2 s).  A wait that reaches it sets
- * the device error word and lets its kernel finish.  No counterpart in the
- * reference, which had no device-side waits of its own. */
+ * the device error word and lets its kernel finish.  b2q_attn_prompt_dev has
+ * waits within a CTA that last as long as its work items: keep the limit
+ * above the time of such a call.  No counterpart in the reference, which had no
+ * device-side waits of its own. */
 b2q_status b2q_set_wait_limit_cycles(b2q_engine* eng, long long cycles);
 
 #ifdef __cplusplus
