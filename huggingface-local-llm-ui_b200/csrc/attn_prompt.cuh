@@ -37,12 +37,14 @@
 // out of f16's subnormals), and the output in TMEM needs no rescaling.  When it
 // does move, the softmax threads rescale the output themselves: the scores'
 // completion covers the P V product issued before them.
-// Values that no row may see reach no result: rows behind a sequence's end are
-// zeroed in shared memory (0 * NaN is NaN), and where a tile with the causal
-// edge holds an infinity or a NaN the CTA computes its rows again one key at a time.
+// Values that a row must not see reach no result (0 * NaN is NaN): in the tiles with the
+// causal edge the rows behind a sequence's end, infinities and NaN are zeroed in shared
+// memory; the rows that do see one of those get it at their end (prompt_show_bad).
 #pragma once
 
 #include <cuda.h>
+
+#include <climits>
 
 #include "attn_paged.cuh"
 #include "gemm_tc.cuh"
@@ -69,35 +71,45 @@ __host__ __device__ constexpr int pr_tile_bytes(int D) { return 128 * D * 2; }  
 __host__ __device__ constexpr int pr_stages(int D) { return D == 128 ? 5 : 8; }
 __host__ __device__ constexpr int pr_smem_bytes(int D) { return (2 + pr_stages(D)) * pr_tile_bytes(D) + 1024; }
 
-// One row (a token's head) by a warp, one key at a time, from global memory.
+// Values that are not finite among the keys k0 .. k1 - 1 of the key tiles that not every
+// row sees whole (there the products took them as zeros): each shows in the rows of the
+// warp that see its key.  The lane's row is `row` (elements from the start of out, < 0:
+// none), its last key `lim`; columns x0 .. x1 - 1 of the head.  A lane looks over the
+// columns lane + 32 e: what matters of one is its first key with +inf and its first with
+// -inf, NaN counting as both, so that the cost is that of reading the tiles once.
 template <int D, typename T>
-__device__ __noinline__ void prompt_row_slow(const PromptArgs& a, int tok, int h, int ka, int last) {
+__device__ __noinline__ void prompt_show_bad(const PromptArgs& a, int ka, int kvh, int k0, int k1, int64_t row, int lim, int x0, int x1) {
   constexpr int E = D / 32;
-  const int lane = threadIdx.x & 31, kvh = h / a.G;
-  float q[E], o[E], m = -INFINITY, sum = 0.0f;
-  const T* qr = reinterpret_cast<const T*>(a.q) + (int64_t)tok * a.q_stride + h * D;
+  const int lane = threadIdx.x & 31;
+  int up[E], down[E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    q[e] = el_f(qr[lane + 32 * e]) * a.scale;
-    o[e] = 0.0f;
+  for (int e = 0; e < E; ++e) up[e] = down[e] = INT_MAX;
+  const T* v = reinterpret_cast<const T*>(a.v) + kvh * D + lane;
+#pragma unroll 4
+  for (int j = k0; j < k1; ++j) {
+    const T* vr = v + (int64_t)(ka + j) * a.v_stride;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float f = el_f(vr[32 * e]);
+      if (!(f < INFINITY)) up[e] = min(up[e], j);
+      if (!(f > -INFINITY)) down[e] = min(down[e], j);
+    }
   }
-  for (int j = 0; j <= last; ++j) {
-    const T* kr = reinterpret_cast<const T*>(a.k) + (int64_t)(ka + j) * a.k_stride + kvh * D;
-    const T* vr = reinterpret_cast<const T*>(a.v) + (int64_t)(ka + j) * a.v_stride + kvh * D;
-    float s = 0.0f;
+  __syncwarp();  // the rows' stores come first
+  for (int y = 0; y < 32; ++y) {
+    const int64_t r = __shfl_sync(B2Q_FULL, row, y);
+    const int l = __shfl_sync(B2Q_FULL, lim, y);
+    if (r < 0) continue;
+    T* o = reinterpret_cast<T*>(a.out) + r + lane;
 #pragma unroll
-    for (int e = 0; e < E; ++e) s = fmaf(q[e], el_f(kr[lane + 32 * e]), s);
-    s = warp_sum(s);
-    const float nm = fmaxf(m, s);  // (a score of -inf has no weight, one that is NaN shows)
-    const float al = m == -INFINITY ? 0.0f : expf(m - nm), p = s == -INFINITY ? 0.0f : expf(s - nm);
-    m = nm;
-    sum = sum * al + p;
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = fmaf(p, el_f(vr[lane + 32 * e]), o[e] * al);
+    for (int e = 0; e < E; ++e) {
+      const bool u = up[e] <= l, d = down[e] <= l;
+      if ((u || d) && lane + 32 * e >= x0 && lane + 32 * e < x1) {
+        const float was = el_f(o[32 * e]);  // (+inf and -inf: NaN; NaN stays)
+        o[32 * e] = el_from<T>(was + (u ? d ? INFINITY - INFINITY : INFINITY : -INFINITY));
+      }
+    }
   }
-  T* orow = reinterpret_cast<T*>(a.out) + ((int64_t)tok * a.H + h) * D;
-#pragma unroll
-  for (int e = 0; e < E; ++e) orow[lane + 32 * e] = el_from<T>(sum == 0.0f ? 0.0f : o[e] / sum);
 }
 
 // ---- tensor copies, matrix and TMEM instructions ----
@@ -184,6 +196,15 @@ __device__ __forceinline__ float pr_exp2(float x) {
 __device__ __forceinline__ float pr_max3(float a, float b, float c) {  // NaN if one is
   float r;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// a * b + c of pairs of 16-bit numbers
+template <bool BF>
+__device__ __forceinline__ uint32_t pr_fma2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  if (BF) asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  else asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
   return r;
 }
 
@@ -474,62 +495,56 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
           sum = w0 * st0.y + w1 * st1.y;
         }
       }
-      if (it.nt > 0 && s_poison[mine & 7] == mine) {
-        for (int y = 0; y < 32; ++y) {
-          if (!__shfl_sync(B2Q_FULL, (int)live, y) || (HALVES && (y & 1) != i)) continue;
-          const int tk = __shfl_sync(B2Q_FULL, tok, y), hh = __shfl_sync(B2Q_FULL, h, y);
-          prompt_row_slow<D, T>(a, it.qa + tk, it.kvh * a.G + hh, it.ka, tk + diff);
-        }
-      } else {
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        // four lanes exchange 16-byte pieces, so that each store writes 64
-        // consecutive bytes of a row: lane y of the four piece y of all four rows
-        const long long at = live ? ((long long)(it.qa + tok) * a.H + it.kvh * a.G + h) * D : -1;
-        long long rows[4];
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      // four lanes exchange 16-byte pieces, so that each store writes 64
+      // consecutive bytes of a row: lane y of the four piece y of all four rows
+      const long long at = live ? ((long long)(it.qa + tok) * a.H + it.kvh * a.G + h) * D : -1;
+      long long rows[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) rows[k] = __shfl_sync(B2Q_FULL, at, (lane & 28) + k);
-        const bool b0 = lane & 1, b1 = lane & 2;
-        const int xa = HALVES ? i * (D / 2) : 0, xe = HALVES ? xa + D / 2 : D;
+      for (int k = 0; k < 4; ++k) rows[k] = __shfl_sync(B2Q_FULL, at, (lane & 28) + k);
+      const bool b0 = lane & 1, b1 = lane & 2;
+      const int xa = HALVES ? i * (D / 2) : 0, xe = HALVES ? xa + D / 2 : D;
 #pragma unroll 1
-        for (int x = xa; x < xe; x += 32) {
-          uint4 v[4];
-          if (it.nt > 0) {
-            uint32_t o[32];
-            pr_ld32((HALVES ? tmem + lane_base + 256 : to) + x, o);
-            pr_wait_ld();
-            if (HALVES) {
+      for (int x = xa; x < xe; x += 32) {
+        uint4 v[4];
+        if (it.nt > 0) {
+          uint32_t o[32];
+          pr_ld32((HALVES ? tmem + lane_base + 256 : to) + x, o);
+          pr_wait_ld();
+          if (HALVES) {
 #pragma unroll
-              for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * w0);
-              if (it.nt > 1) {
-                uint32_t o1[32];
-                pr_ld32(tmem + lane_base + 256 + D + x, o1);
-                pr_wait_ld();
+            for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * w0);
+            if (it.nt > 1) {
+              uint32_t o1[32];
+              pr_ld32(tmem + lane_base + 256 + D + x, o1);
+              pr_wait_ld();
 #pragma unroll
-                for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(fmaf(__uint_as_float(o1[y]), w1, __uint_as_float(o[y])));
-              }
+              for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(fmaf(__uint_as_float(o1[y]), w1, __uint_as_float(o[y])));
             }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              uint32_t w[4];
-#pragma unroll
-              for (int y = 0; y < 4; ++y)
-                w[y] = el_pack2<T>(__uint_as_float(o[8 * k + 2 * y]) * inv, __uint_as_float(o[8 * k + 2 * y + 1]) * inv);
-              v[k] = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-          } else {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] = make_uint4(0u, 0u, 0u, 0u);
           }
-          pr_swap(b0, 1, v[0], v[1]);
-          pr_swap(b0, 1, v[2], v[3]);
-          pr_swap(b1, 2, v[0], v[2]);
-          pr_swap(b1, 2, v[1], v[3]);
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (rows[k] >= 0) *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + rows[k] + x + (lane & 3) * 8) = v[k];
+          for (int k = 0; k < 4; ++k) {
+            uint32_t w[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+              w[y] = el_pack2<T>(__uint_as_float(o[8 * k + 2 * y]) * inv, __uint_as_float(o[8 * k + 2 * y + 1]) * inv);
+            v[k] = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[k] = make_uint4(0u, 0u, 0u, 0u);
         }
-        tc_fence_before();  // (the output's reads come before the next item's first product)
+        pr_swap(b0, 1, v[0], v[1]);
+        pr_swap(b0, 1, v[2], v[3]);
+        pr_swap(b1, 2, v[0], v[2]);
+        pr_swap(b1, 2, v[1], v[3]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (rows[k] >= 0) *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + rows[k] + x + (lane & 3) * 8) = v[k];
       }
+      tc_fence_before();  // (the output's reads come before the next item's first product)
+      if (it.nt > 0 && s_poison[mine & 7] == mine)
+        prompt_show_bad<D, T>(a, it.ka, it.kvh, it.kt_edge * kPrN, min(it.l, it.nt * kPrN), at, lim, xa, xe);
       if (HALVES && it.nt > 0) {  // (which reads no probabilities of this half)
         __syncwarp();
         if (lane == 0) mbar_arrive(&o_free);
@@ -704,7 +719,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
           if (!ok) break;
           land ^= 1u << st;
           uint8_t* vt = ring + st * TB;
-          bool bad = false;
+          uint32_t nan = 0;  // (pairs) the sum of 0 * value: NaN if one is not finite
 #pragma unroll
           for (int hh = 0; hh < 2; ++hh) {
             const int row = w + 64 * hh;
@@ -712,18 +727,22 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
               for (int y = 0; y < 8 * NC; ++y)
                 *reinterpret_cast<uint4*>(vt + (y >> 3) * CB + row * 128 + ((y ^ row) & 7) * 16) = make_uint4(0, 0, 0, 0);
             } else {
-              // an infinity or NaN has all exponent bits set
-              constexpr uint32_t em = BF ? 0x7f80u : 0x7c00u;
-#pragma unroll 4
+#pragma unroll
               for (int y = 0; y < 8 * NC; ++y) {
                 const uint4 v = *reinterpret_cast<const uint4*>(vt + (y >> 3) * CB + row * 128 + ((y ^ row) & 7) * 16);
-                const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int z = 0; z < 4; ++z) bad = bad || (u[z] & em) == em || (u[z] & (em << 16)) == (em << 16);
+                nan = pr_fma2<BF>(v.x, 0u, pr_fma2<BF>(v.y, 0u, pr_fma2<BF>(v.z, 0u, pr_fma2<BF>(v.w, 0u, nan))));
               }
             }
           }
-          if (__any_sync(B2Q_FULL, bad)) s_poison[count & 7] = count;
+          if (__any_sync(B2Q_FULL, (nan & 0x7fff7fffu) != 0)) {
+            s_poison[count & 7] = count;
+            constexpr uint32_t em = BF ? 0x7f80u : 0x7c00u;  // an infinity or NaN has all exponent bits set
+#pragma unroll 1
+            for (int x = 0; x < 2 * 32 * NC; ++x) {  // two values of row w or w + 64 (in whatever order)
+              uint32_t* u = reinterpret_cast<uint32_t*>(vt + (x >> 6) * CB + (w + 64 * (x >> 5 & 1)) * 128) + (x & 31);
+              *u &= ((*u & em) == em ? 0u : 0xffffu) | ((*u & (em << 16)) == (em << 16) ? 0u : 0xffff0000u);
+            }
+          }
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) mbar_arrive(&v_ok[st]);

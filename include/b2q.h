@@ -426,7 +426,8 @@ typedef struct {
 /* Causal attention of packed prompts, query heads grouped as above.  out
  * [n_q][n_heads * head_dim] contiguous; rows from q_start[n_seqs] on are left
  * as they are, queries without keys give zeros.  0 < scale <= 1e30.  Scores, sums and outputs are
- * accumulated in f32, the probabilities rounded to `type`. */
+ * accumulated in f32, the probabilities rounded to `type`.  A value that is infinite or NaN
+ * shows as such in the queries that attend its key, and in no other. */
 b2q_status b2q_attn_prompt_dev(b2q_engine* eng, const b2q_prompt* p, const void* q, int64_t q_stride, const void* k,
                                int64_t k_stride, const void* v, int64_t v_stride, float scale, void* out, void* stream);
 
