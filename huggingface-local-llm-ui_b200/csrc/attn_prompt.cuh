@@ -752,6 +752,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
       if (!ok) *s_fail = 1;
     }
   }
+  kv_check_offsets(a.q_start, a.n_seqs, s_q[0], s_q + 1, cached);
   __syncwarp();
   tc_fence_before();
   __syncthreads();

@@ -250,15 +250,32 @@ __device__ __forceinline__ void kv_store_row(uint8_t* blk, int tok, const float 
   }
 }
 
+// By all threads of the grid: offsets that decrease set the error word (beside them the
+// search for a row's sequence may miss rows).  `first` and `s_ends`: the CTA's copies of
+// start[0] and start[1..n_seqs], where `cached`.
+__device__ __forceinline__ void kv_check_offsets(const int32_t* start, int n_seqs, int first, const int* s_ends, bool cached) {
+  constexpr unsigned kCtas = 256;  // (that share the work)
+  if (cached) {
+    if (blockIdx.x == 0 && blockIdx.y == 0)
+      for (int i = threadIdx.x; i < n_seqs; i += blockDim.x)
+        if (s_ends[i] < (i ? s_ends[i - 1] : first)) kv_batch_error();
+  } else if (blockIdx.x < kCtas && blockIdx.y == 0) {
+    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < n_seqs; i += min(gridDim.x, kCtas) * blockDim.x)
+      if (start[i + 1] < start[i]) kv_batch_error();
+  }
+}
+
 // Sequences of a batch whose offsets are copied to shared memory to be searched.
 constexpr int kKvSeqs = 1024;
 
 // By the first `rows` threads of a CTA: block and position of packed rows
-// row0 .. row0 + rows - 1 (block -1: no row); s_start: [kKvSeqs].
+// row0 .. row0 + rows - 1 (block -1: no row); s_start: [kKvSeqs + 1] for the sequences'
+// ends and, last, the first one's start.
 __device__ __forceinline__ void kv_rows_of(const KvBatch& b, int row0, int rows, int* s_start, int64_t* s_blk, int* s_pos) {
   const bool in_smem = b.n_seqs <= kKvSeqs;
   if (in_smem) {
     for (int i = threadIdx.x; i < b.n_seqs; i += blockDim.x) s_start[i] = b.q_start[i + 1];
+    if (threadIdx.x == blockDim.x - 1) s_start[kKvSeqs] = b.q_start[0];
     __syncthreads();
   }
   if ((int)threadIdx.x < rows) {
@@ -304,7 +321,7 @@ __global__ void __launch_bounds__(kAppendThreads, 4) kv_append_kernel(const __gr
   constexpr int L = D / 4, RW = 32 / L, W = kAppendThreads / 32;
   constexpr int NU = TOK == 1 ? 2 : 1, NI = NU * TOK;  // turns (RW rows) taken together, rows in registers
   __shared__ int64_t s_blk[TOK];
-  __shared__ int s_pos[TOK], s_start[kKvSeqs];
+  __shared__ int s_pos[TOK], s_start[kKvSeqs + 1];
   pdl_wait();
   pdl_launch_dependents();
   const int t0 = blockIdx.x * TOK;
@@ -339,6 +356,7 @@ __global__ void __launch_bounds__(kAppendThreads, 4) kv_append_kernel(const __gr
     kv_batch_error();
     s_blk[threadIdx.x] = -1;
   }
+  kv_check_offsets(a.b.q_start, a.b.n_seqs, s_start[kKvSeqs], s_start, a.b.n_seqs <= kKvSeqs);
   __syncthreads();
   const int bpp = a.b.page_tokens / kKvBlk;
   auto turn = [&](auto kind_c, int u, float (&v)[4], int j) {  // row `sub` of turn u of the kind, token j
@@ -423,7 +441,7 @@ __global__ void __launch_bounds__(256) kv_gather_kernel(const __grid_constant__ 
   typedef typename Elem<OT>::type O;
   constexpr int NB = D / 32;
   __shared__ int64_t s_blk[kGatherRows];  // block of head 0, -1: no row
-  __shared__ int s_pos[kGatherRows], s_start[kKvSeqs];
+  __shared__ int s_pos[kGatherRows], s_start[kKvSeqs + 1];
   pdl_wait();
   pdl_launch_dependents();
   const int row0 = blockIdx.x * kGatherRows;
@@ -473,6 +491,7 @@ __global__ void __launch_bounds__(256) kv_gather_kernel(const __grid_constant__ 
       }
     }
   }
+  kv_check_offsets(a.b.q_start, a.b.n_seqs, s_start[kKvSeqs], s_start, a.b.n_seqs <= kKvSeqs);
 }
 
 }  // namespace b2q

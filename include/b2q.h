@@ -324,8 +324,9 @@ b2q_status b2q_gdn_step_dev(b2q_engine* eng, const b2q_gdn_config* cfg, int n_to
  * The device arrays of a batch are not trusted: a position, page or offset
  * out of range is skipped (a row that has no valid place is not written, a
  * key with no valid page is not attended) and b2q_check_device_error()
- * returns B2Q_EINVAL once.  A decreasing offset leaves its sequence without
- * rows. */
+ * returns B2Q_EINVAL once.  So it does for an offset that decreases: its
+ * sequence has no rows, and rows of other sequences may be left as they
+ * are. */
 typedef struct {
   int n_heads;     /* query heads, a multiple of n_kv_heads, at most 1024 */
   int n_kv_heads;

@@ -135,3 +135,42 @@ def test_rows_without_a_position_are_left_as_they_are(engine, pkg, q_type, pages
     # the sequence's keys are those of the table, whatever kv_len claims
     for claimed in (cap + 1, cap + 3, cap + 4, cap + 100, 2 ** 31 - 1, 3, 1, 0, -1, -2 ** 31):
         rows_left(engine, pool, ks, vs, q, q_type, claimed, cap)
+
+
+def offsets_reported(engine, f):
+    from hf_llm_b200._lib import B2QError, EINVAL
+    f()
+    torch.cuda.synchronize()
+    with pytest.raises(B2QError) as e:
+        engine.check_device_error()
+    assert e.value.status == EINVAL
+    engine.check_device_error()
+
+
+@pytest.mark.parametrize("seqs", [2, 150, 1500])
+def test_offsets_that_decrease_are_reported(engine, pkg, seqs):
+    """By each of the four calls, also where no row of the call falls into the
+    sequence that they belong to."""
+    from hf_llm_b200 import paged
+    start = [0] * (seqs - 1) + [3, 2]
+    H, KV, D, st = 4, 2, 64, 1
+    cfg = paged.kv_config(H, KV, D, R.Q4_0, 16, seqs, 1)
+    qs = torch.tensor(start, dtype=torch.int32).cuda()
+    lens = torch.full((seqs,), 16, dtype=torch.int32).cuda()
+    tab = torch.arange(seqs, dtype=torch.int32).cuda()
+    pages = torch.zeros(seqs * paged.page_bytes(cfg), dtype=torch.uint8, device="cuda")
+    b = paged.kv_batch(seqs, 4, 3, qs.data_ptr(), lens.data_ptr(), tab.data_ptr())
+    q, k, v = (rand((4, h, D), i, F16).cuda() for i, h in enumerate((H, KV, KV)))
+    out = torch.empty_like(q)
+    work = torch.empty(engine.attn_paged_work_bytes(cfg, b), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    engine.check_device_error()
+    offsets_reported(engine, lambda: engine.kv_append_dev(cfg, b, None, F16, q.data_ptr(), H * D, k.data_ptr(), KV * D, v.data_ptr(), KV * D,
+                                                          pages.data_ptr(), out.data_ptr(), F16, st))
+    offsets_reported(engine, lambda: engine.kv_gather_dev(cfg, b, pages.data_ptr(), k.data_ptr(), v.data_ptr(), F16, st))
+    offsets_reported(engine, lambda: engine.attn_paged_dev(cfg, b, q.data_ptr(), F16, H * D, pages.data_ptr(), 0.1, out.data_ptr(), F16,
+                                                           work.data_ptr(), work.numel(), st))
+    ks = torch.tensor([0] * seqs + [4], dtype=torch.int32).cuda()
+    p = paged.prompt(H, KV, D, F16, seqs, 4, 4, 3, qs.data_ptr(), ks.data_ptr())
+    offsets_reported(engine, lambda: engine.attn_prompt_dev(p, q.data_ptr(), H * D, k.data_ptr(), KV * D, v.data_ptr(), KV * D, 0.1,
+                                                            out.data_ptr(), st))
