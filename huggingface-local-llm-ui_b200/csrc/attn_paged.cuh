@@ -527,8 +527,8 @@ __global__ void __launch_bounds__(PgThreads<NG>::value, 1) attn_paged_kernel(con
       if (am == 0.0f || e >= 127) e = 13;
       e = max(e, -100);
       const float sc = __uint_as_float((uint32_t)(127 + 13 - e) << 23);
-      // and never 0, which would undo the mask's -inf
-      fac[n] = fmaxf(a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)(127 - 13 + e) << 23), 1e-37f);
+      // and never 0, which would undo the mask's -inf, nor infinite: a product of 0 stays 0
+      fac[n] = fminf(fmaxf(a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)(127 - 13 + e) << 23), 1e-37f), 3e38f);
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll

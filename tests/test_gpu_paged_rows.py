@@ -174,3 +174,17 @@ def test_offsets_that_decrease_are_reported(engine, pkg, seqs):
     p = paged.prompt(H, KV, D, F16, seqs, 4, 4, 3, qs.data_ptr(), ks.data_ptr())
     offsets_reported(engine, lambda: engine.attn_prompt_dev(p, q.data_ptr(), H * D, k.data_ptr(), KV * D, v.data_ptr(), KV * D, 0.1,
                                                             out.data_ptr(), st))
+
+
+def test_scores_of_zero_under_a_large_scale(engine, pkg):
+    """Keys of zeros under queries and a scale whose product passes f32's range: all
+    scores are 0, and the output is the values' mean."""
+    pool = Pool(4, 2, 64, 16, [50], [1])
+    ks, vs = pool.fill()
+    scale_tokens(pool, 0, range(50), 0.0, keys=True)
+    q = torch.full((1, 4, 64), 1e20)
+    out = run_paged(engine, pool.upload(), q, F32, F32, 1e30)
+    mean = torch.from_numpy(vs[0].mean(0)).repeat_interleave(2, 0)[None]
+    # two parts of each probability times scale, 2^-21, and eight f32 roundings on the way out
+    R.check_close(out, mean, torch.full_like(mean, 2.0 ** -20 * float(np.abs(vs[0]).max())))
+    engine.check_device_error()
