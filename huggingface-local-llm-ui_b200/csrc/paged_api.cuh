@@ -175,7 +175,6 @@ static bool prompt_map_q(CUtensorMap* m, const PromptArgs& a, int D, int type) {
   return prompt_map(m, type, 4, a.q, dims, strides, box);
 }
 static bool prompt_map_kv(CUtensorMap* m, const void* p, int64_t stride, int rows, int KV, int D, int type) {
-  if (rows == 0) return true;  // (no tile is loaded)
   const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)KV, (cuuint64_t)rows};
   const cuuint64_t strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)stride * 2};
   const cuuint32_t box[3] = {64u, 1u, (cuuint32_t)kPrN};
@@ -429,8 +428,10 @@ b2q_status b2q_attn_prompt_dev(b2q_engine* e, const b2q_prompt* p, const void* q
   a.chunks = (a.G + a.gp - 1) / a.gp;
   a.tpt = kPrM / a.gp;
   CUtensorMap mq, mk, mv;
-  if (!prompt_map_q(&mq, a, D, t) || !prompt_map_kv(&mk, a.k, a.k_stride, a.n_kv, a.KV, D, t) ||
-      !prompt_map_kv(&mv, a.v, a.v_stride, a.n_kv, a.KV, D, t))
+  bool maps = prompt_map_q(&mq, a, D, t);
+  if (a.n_kv == 0) mk = mv = mq;  // (no tile is loaded, but the kernel prefetches all three)
+  else maps = maps && prompt_map_kv(&mk, a.k, a.k_stride, a.n_kv, a.KV, D, t) && prompt_map_kv(&mv, a.v, a.v_stride, a.n_kv, a.KV, D, t);
+  if (!maps)
     return set_error(B2Q_ECUDA, "%s: cuTensorMapEncodeTiled failed", what);
   // two row tiles to an item; one, in halves, where those are no more than the SMs
   // (16 tokens behind 2048: 23 us, 32 with room for a second row tile; with more items

@@ -70,3 +70,14 @@ def test_a_bad_value_behind_a_long_prefix_holds_nothing_up(engine, pkg, type_, a
             out = run_prompt(engine, heads, kv, dim, type_, [n], [l], q, k, v, 0.1)
             engine.check_device_error()
             expect(out, zeroed, v, heads, [n], [l])
+
+
+@pytest.mark.parametrize("type_", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_no_keys_in_the_call(engine, pkg, type_, dim):
+    """n_kv = 0, with NULL keys and values: zeros."""
+    q = rand((40, 4, dim), 1, type_)
+    none = torch.empty(0, 2, dim, dtype=TYPES[type_])
+    out = run_prompt(engine, 4, 2, dim, type_, [30, 0, 10], [0, 0, 0], q, none, none, 0.1)
+    assert (out == 0).all()
+    engine.check_device_error()
