@@ -296,9 +296,9 @@ b2q_status b2q_kv_gather_dev(b2q_engine* e, const b2q_kv_config* cfg, const b2q_
 }
 
 size_t b2q_attn_paged_work_bytes(const b2q_engine* e, const b2q_kv_config* cfg, const b2q_kv_batch* batch) {
-  if (!e || check_kv_config("b2q_attn_paged_work_bytes", cfg) != B2Q_OK ||
-      check_kv_batch("b2q_attn_paged_work_bytes", batch) != B2Q_OK)
-    return 0;
+  static const char* const what = "b2q_attn_paged_work_bytes";
+  if (!e) set_error(B2Q_EINVAL, "%s: NULL engine", what);
+  if (!e || check_kv_config(what, cfg) != B2Q_OK || check_kv_batch(what, batch) != B2Q_OK) return 0;
   // descriptors and pieces of the items cut between CTAs (16 rows: either tiling)
   const size_t ctas = paged_ctas(e), D = cfg->head_dim;
   return paged_desc_bytes(ctas) + ctas * 2 * pg_part_floats(D, 2) * sizeof(float) +

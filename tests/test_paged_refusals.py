@@ -114,3 +114,15 @@ def test_empty_batches_do_nothing(calls):
 def test_page_bytes(calls):
     assert calls["paged"].page_bytes(calls["cfg"]()) == 2 * 4 * 18 * 128
     assert calls["paged"].page_bytes(calls["cfg"](head_dim=64, page_tokens=16, n_kv_heads=8)) == 8 * 18 * 64
+
+
+def test_workspace_of_bad_arguments(calls):
+    """0, and a text of its own rather than the last failure's."""
+    work = calls["lib"].b2q_attn_paged_work_bytes
+    for e, c, b, text in ((None, calls["cfg"](), calls["batch"](), "engine"), (calls["keep"], calls["cfg"](n_heads=7), calls["batch"](), "heads"),
+                          (calls["keep"], calls["cfg"](), calls["batch"](kv_len=None), "NULL array")):
+        assert calls["prompt"](type=Q4_0) == 6  # another failure first
+        assert work(e and C.cast(e, C.c_void_p), c, b) == 0
+        said = calls["lib"].b2q_last_error().decode()
+        assert "b2q_attn_paged_work_bytes" in said and text in said
+    assert work(C.cast(calls["keep"], C.c_void_p), calls["cfg"](), calls["batch"]()) > 0
