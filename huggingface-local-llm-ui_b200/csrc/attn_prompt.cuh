@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
   constexpr int NC = D / 64;
   constexpr bool BF = TYPE == kElBF16;
   extern __shared__ uint8_t pr_smem[];
-  __shared__ uint64_t q_full[2], q_empty[2], full[NS], empty[NS], v_land[NS], v_ok[NS], s_full[2], p_full[2], o_full[2], x_full, o_free, done;
+  __shared__ uint64_t q_full[2], q_empty[2], full[NS], empty[NS], v_land[NS], v_ok[NS], s_full[2], p_full[2], o_full[2], x_full, done;
   __shared__ uint32_t s_tmem;
   __shared__ int s_fail_, s_poison_[8], s_q[kPrSeqs + 1], s_k[kPrSeqs + 1];
   volatile int *s_fail = &s_fail_, *s_poison = s_poison_;
@@ -289,7 +289,6 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
       mbar_init(&v_ok[i], 2);
     }
     mbar_init(&x_full, 8);
-    mbar_init(&o_free, 8);
     mbar_init(&done, 1);
     *s_fail = 0;
     for (int i = 0; i < 8; ++i) s_poison[i] = 0;
@@ -360,19 +359,20 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
     it.kt_edge = lim < 0 ? 0 : (lim + 1) / kPrN;
     return true;
   };
-  const int rounds = (a.items + (int)gridDim.x - 1) / (int)gridDim.x;
+  // (in halves there are no more items than CTAs)
+  const int rounds = HALVES ? 1 : (a.items + (int)gridDim.x - 1) / (int)gridDim.x;
 
   if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     // ---- softmax of row tile i, or of every second key tile ----
     const int i = warp >> 2, ir = HALVES ? 0 : i, r = threadIdx.x & 127;
-    float2* s_stat = reinterpret_cast<float2*>(qs + TB);  // [2][2][128] (halves: no second query tile): reference, sum
+    float2* s_stat = reinterpret_cast<float2*>(qs + TB);  // [2][128] (halves: no second query tile): reference, sum
     const int tr = fdiv(r, a.d_gp), hr = r - tr * a.gp;  // the row's token and head within the tile
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + lane_base + i * 128, to = tmem + lane_base + 256 + i * D;
     const float c = a.scale * 1.4426950408889634f;
     const f2 c2 = f2_of(c, c);
-    uint32_t s_ph = 0, o_ph = 0, x_ph = 0;  // (o_ph: a bit for each half)
+    uint32_t s_ph = 0, o_ph = 0;
     int count = 0;  // items with key tiles, of either row tile
     bool ok = true;
     int round = -1;
@@ -470,25 +470,18 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
       float w0 = 1.0f, w1 = 0.0f;  // weights of the halves' outputs
       if (it.nt > 0) {
         // (in halves both outputs; a second one where there are two key tiles)
-        ok = __all_sync(B2Q_FULL, mbar_wait_bounded(&o_full[ir], o_ph & 1)) && !*s_fail;
+        ok = __all_sync(B2Q_FULL, mbar_wait_bounded(&o_full[ir], o_ph)) && !*s_fail;
         o_ph ^= 1;
-        if (HALVES && ok && it.nt > 1) {
-          ok = __all_sync(B2Q_FULL, mbar_wait_bounded(&o_full[1], o_ph >> 1)) && !*s_fail;
-          o_ph ^= 2;
-        }
+        if (HALVES && ok && it.nt > 1) ok = __all_sync(B2Q_FULL, mbar_wait_bounded(&o_full[1], 0)) && !*s_fail;
         if (!ok) break;
         tc_fence_after();
         if (HALVES) {
-          // both halves meet at each item, so that the two places for what they
-          // tell one another (x_ph) are free again when they are next written
-          float2* stat = s_stat + x_ph * 256;
-          stat[128 * i + r] = make_float2(ref, sum);
+          s_stat[128 * i + r] = make_float2(ref, sum);
           __syncwarp();
           if (lane == 0) mbar_arrive(&x_full);
-          ok = __all_sync(B2Q_FULL, mbar_wait_bounded(&x_full, x_ph)) && !*s_fail;
+          ok = __all_sync(B2Q_FULL, mbar_wait_bounded(&x_full, 0)) && !*s_fail;
           if (!ok) break;
-          x_ph ^= 1;
-          const float2 st0 = stat[r], st1 = stat[128 + r];
+          const float2 st0 = s_stat[r], st1 = s_stat[128 + r];
           const float top = fmaxf(st0.x, st1.x);
           w0 = st0.x == -INFINITY ? 0.0f : pr_exp2(st0.x - top);
           w1 = st1.x == -INFINITY ? 0.0f : pr_exp2(st1.x - top);
@@ -545,10 +538,6 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
       tc_fence_before();  // (the output's reads come before the next item's first product)
       if (it.nt > 0 && s_poison[mine & 7] == mine)
         prompt_show_bad<D, T>(a, it.ka, it.kvh, it.kt_edge * kPrN, min(it.l, it.nt * kPrN), at, lim, xa, xe);
-      if (HALVES && it.nt > 0) {  // (which reads no probabilities of this half)
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&o_free);
-      }
       it = nx;
     }
     if (!ok) *s_fail = 1;
@@ -635,7 +624,6 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
         }
         pr_commit(&s_full[i]);
       };
-      uint32_t o_ph = 1;  // of o_free: the first item waits for none
       for (int round = 0; ok && round < rounds; ++round) {
         PrItem it;
         if (!item(round, it) || it.nt == 0) continue;
@@ -671,10 +659,6 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
           if (ok && more) {
             ok = wait(&full[sk], ph);
             next();
-          }
-          if (ok && HALVES && j == 0) {  // both halves have read the last item's outputs
-            ok = wait(&o_free, o_ph);
-            o_ph ^= 1;
           }
           const int ie = HALVES ? (j & 1) + 1 : it.nq;
           for (int i = HALVES ? j & 1 : 0; ok && i < ie; ++i) {
