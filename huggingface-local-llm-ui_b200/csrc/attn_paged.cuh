@@ -34,7 +34,7 @@
 // the matrix unit aligns products by their nominal exponents: 2^-17 is lost.)
 // A row's softmax reference follows the largest p_j * scale_j of the keys that the row
 // sees (the largest scale of a key's blocks of dims) in steps of 2^8, so that it lies
-// between 2^7 and 2^15: a product keeps its bits down to 2^-32 of that one (f16's
+// between 2^6 and 2^15: a product keeps its bits down to 2^-31 of that one (f16's
 // smallest step is 2^-24), and outputs are seldom rescaled.
 #pragma once
 
@@ -215,12 +215,6 @@ __device__ __forceinline__ int pg_keys(const PagedArgs& a, const PgAt& p) {
 __device__ __forceinline__ float pg_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-__device__ __forceinline__ float pg_log2(float x) {
-  float y;
-  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -561,9 +555,12 @@ __global__ void __launch_bounds__(PgThreads<NG>::value, 1) attn_paged_kernel(con
   // half of the time) ----
   auto tile = [&](const uint8_t* tb, uint32_t vm) {
     const int key0 = at_blk * kKvBlk;
-    // log2 of the largest value scale of tokens 2 lane and 2 lane + 1 of the tile.  (The
-    // larger of a number and NaN is the number; what is not finite, or zero, counts as
-    // the nearest scale that is, and shows in the products.)
+    // Exponent of the largest value scale of tokens 2 lane and 2 lane + 1 of the tile.  (A
+    // whole number: a row whose reference it moves has a power of two for its largest
+    // probability, whose products with the f16 scales are exact; with the logarithm itself
+    // f16 outputs were off by 2.65e-4, not 2.45e-4.  The larger of a number and NaN is the
+    // number; what is not finite, or zero, counts as the nearest scale that is, and shows
+    // in the products.)
     float lg[2];
     {
       const int blk = lane >> 3;
@@ -583,7 +580,7 @@ __global__ void __launch_bounds__(PgThreads<NG>::value, 1) attn_paged_kernel(con
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const float2 f = __half22float2(u32_h2(m[e]));
-        lg[e] = pg_log2(fminf(fmaxf(fmaxf(f.x, f.y), 0x1p-24f), 65504.0f));
+        lg[e] = (float)(int)(__float_as_uint(fminf(fmaxf(fmaxf(f.x, f.y), 0x1p-24f), 65504.0f)) >> 23) - 127.0f;
       }
     }
     float ta[NG][D / 16][4];
@@ -657,8 +654,8 @@ __global__ void __launch_bounds__(PgThreads<NG>::value, 1) attn_paged_kernel(con
             }
       }
       // softmax: the reference moves when a product of a probability and a value scale
-      // that the row sees has outgrown it by 2^15 (the largest product since it last
-      // moved is 2^7 or above)
+      // that the row sees may have outgrown it by 2^15 (when it moves, the largest
+      // product is 2^6 or above)
       float sl[2][2];
 #pragma unroll
       for (int x = 0; x < 2; ++x)
@@ -671,14 +668,14 @@ __global__ void __launch_bounds__(PgThreads<NG>::value, 1) attn_paged_kernel(con
                          fmaxf(fmaf(s[n][1][0], fac[n], sl[1][0]), fmaf(s[n][1][1], fac[n], sl[1][1])));
         tm = fmaxf(tm, __shfl_xor_sync(B2Q_FULL, tm, 1));
         mx[n] = fmaxf(mx[n], fmaxf(tm, __shfl_xor_sync(B2Q_FULL, tm, 2)));
-        move = move || mx[n] - 15.0f > ref[n];
+        move = move || mx[n] - 14.0f > ref[n];
       }
       if (__any_sync(B2Q_FULL, move)) {
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
           float cr = 1.0f;
-          if (mx[n] - 15.0f > ref[n]) {
-            const float nref = mx[n] - 7.0f;
+          if (mx[n] - 14.0f > ref[n]) {
+            const float nref = mx[n] - 6.0f;
             cr = pg_weight(ref[n], nref);
             ref[n] = nref;
           }

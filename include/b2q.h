@@ -400,7 +400,7 @@ b2q_status b2q_kv_gather_dev(b2q_engine* eng, const b2q_kv_config* cfg, const b2
  * Sums and the softmax in f32; f32 queries are carried as two f16 parts
  * (~2^-22), and so is a probability times its value's scale where out is f32;
  * for 16-bit outputs that product is rounded once, to f16.  Beside that such a
- * product is off by at most 2^-32 of the row's largest one.  0 < scale <=
+ * product is off by at most 2^-31 of the row's largest one.  0 < scale <=
  * 1e30.  out [n_tokens][n_heads * head_dim] contiguous.  Offsets that go up and
  * down until the sequences' rows are many times the batch's: nothing is done.
  * `work`: at least b2q_attn_paged_work_bytes() (16-byte aligned; no initial

@@ -37,8 +37,8 @@ def value_scales(pool, s):
 
 def check_rows(out, pool, ks, vs, q, scale, q_type, out_type):
     """Each row against f64 by itself.  A probability times its value's scale enters as
-    f16, one part or two, and the largest such product that the row has is 2^7 or above: a
-    term is off by 2^-25 (half of f16's smallest step) beside its relative error, so by 2^-32
+    f16, one part or two, and the largest such product that the row has is 2^6 or above: a
+    term is off by 2^-25 (half of f16's smallest step) beside its relative error, so by 2^-31
     of that product, times |code - 8| <= 8.  (1.02: the kernel's own probabilities.)"""
     G, a = pool.H // pool.KV, 0
     for s, n in enumerate(pool.news):
@@ -50,7 +50,7 @@ def check_rows(out, pool, ks, vs, q, scale, q_type, out_type):
                 w = torch.from_numpy(ks[s][:see, h // G]) @ x[h] * scale
                 m = float((torch.softmax(w, 0) * torch.from_numpy(top[:see, h // G])).max())
                 want, bound = R.attend(x[None, h:h + 1], [ks[s][:see, h // G:h // G + 1]], [vs[s][:see, h // G:h // G + 1]], [1], scale,
-                                       TYPES[out_type], E_SCORE, e_prob(out_type), 1.02 * 2.0 ** -29 * m)
+                                       TYPES[out_type], E_SCORE, e_prob(out_type), 1.02 * 2.0 ** -28 * m)
                 R.check_close(out[a + i:a + i + 1, h:h + 1], want, bound)
         a += n
 
