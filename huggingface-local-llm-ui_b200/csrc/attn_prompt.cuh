@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
   extern __shared__ uint8_t pr_smem[];
   __shared__ uint64_t q_full[2], q_empty[2], full[NS], empty[NS], v_land[NS], v_ok[NS], s_full[2], p_full[2], o_full[2], x_full, done;
   __shared__ uint32_t s_tmem;
-  __shared__ int s_fail_, s_poison_[8], s_q[kPrSeqs + 1], s_k[kPrSeqs + 1];
+  __shared__ int s_fail_, s_poison_[16], s_q[kPrSeqs + 1], s_k[kPrSeqs + 1];
   volatile int *s_fail = &s_fail_, *s_poison = s_poison_;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pr_smem) + 1023) & ~(uintptr_t)1023);
@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
     mbar_init(&x_full, 8);
     mbar_init(&done, 1);
     *s_fail = 0;
-    for (int i = 0; i < 8; ++i) s_poison[i] = 0;
+    for (int i = 0; i < 16; ++i) s_poison[i] = 0;
     fence_mbar_init();
   }
   if (warp == 8 && lane == 0) {
@@ -373,14 +373,15 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
     const float c = a.scale * 1.4426950408889634f;
     const f2 c2 = f2_of(c, c);
     uint32_t s_ph = 0, o_ph = 0;
-    int count = 0;  // items with key tiles, of either row tile
+    int count = 0;  // items with key tiles and this row tile
     bool ok = true;
     int round = -1;
     auto next_item = [&](PrItem& it) {  // the next item with this row tile
       while (++round < rounds) {
         if (!item(round, it)) continue;
+        if (ir >= it.nq) continue;
         if (it.nt > 0) ++count;
-        if (ir < it.nq) return true;
+        return true;
       }
       return false;
     };
@@ -536,7 +537,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
           if (rows[k] >= 0) *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + rows[k] + x + (lane & 3) * 8) = v[k];
       }
       tc_fence_before();  // (the output's reads come before the next item's first product)
-      if (it.nt > 0 && s_poison[mine & 7] == mine)
+      if (it.nt > 0 && s_poison[8 * ir + (mine & 7)] == mine)
         prompt_show_bad<D, T>(a, it.ka, it.kvh, it.kt_edge * kPrN, min(it.l, it.nt * kPrN), at, lim, xa, xe);
       it = nx;
     }
@@ -691,12 +692,16 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
       // ---- value tiles that some row sees only in part ----
       const int w = threadIdx.x - 320;  // 0..63: rows w and w + 64
       uint32_t land = 0;
-      int x0 = 0, count = 0;  // the item's first stage, items with key tiles
+      // The item's first stage; items with key tiles of either row tile, in eight places for
+      // each: the ring ends a few items ahead of a row tile's own next one, but row tile 0
+      // may go through any number of items that have no second one while that one ends.
+      int x0 = 0, count[2] = {0, 0};
       bool ok = true;
       for (int round = 0; ok && round < rounds; ++round) {
         PrItem it;
         if (!item(round, it) || it.nt == 0) continue;
-        ++count;
+        ++count[0];
+        count[1] += it.nq == 2;
         for (int j = it.kt_edge; j < it.nt; ++j) {
           const int st = (x0 + (HALVES && j + 1 < it.nt ? 2 * j + 2 : 2 * j + 1)) % NS;
           ok = __all_sync(B2Q_FULL, mbar_wait_bounded(&v_land[st], (land >> st) & 1)) && !*s_fail;
@@ -719,7 +724,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid
             }
           }
           if (__any_sync(B2Q_FULL, (nan & 0x7fff7fffu) != 0)) {
-            s_poison[count & 7] = count;
+            s_poison[count[0] & 7] = count[0];
+            if (it.nq == 2) s_poison[8 + (count[1] & 7)] = count[1];
             constexpr uint32_t em = BF ? 0x7f80u : 0x7c00u;  // an infinity or NaN has all exponent bits set
 #pragma unroll 1
             for (int x = 0; x < 2 * 32 * NC; ++x) {  // two values of row w or w + 64 (in whatever order)

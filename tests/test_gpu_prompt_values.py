@@ -41,6 +41,8 @@ def expect(out, zeroed, v, heads, news, lens):
     (6, 1, 64, [129], [1000], 0.02),
     (32, 8, 128, [500, 310, 64], [500, 900, 64], 1e-4),  # several items a CTA
     (1, 1, 128, [70], [70], 1.0),                        # nothing is finite
+    # many items with one row tile between those with two
+    (64, 8, 64, [1 + 7 * i % 41 for i in range(80)], [1 + 7 * i % 41 + 97 * i % 300 for i in range(80)], 1e-3),
 ])
 def test_bad_values_anywhere(engine, pkg, type_, heads, kv, dim, news, lens, share):
     q, k, v = (rand((sum(x), h, dim), s, type_) for s, (x, h) in enumerate(((news, heads), (lens, kv), (lens, kv))))
