@@ -6,9 +6,10 @@
 // that stream is the floor.  What bounds the kernel is the instructions beside it
 // (some 530 a warp for 16 keys and 16 rows, half of them unpacking), issued on 43 to
 // 52 % of the cycles: two or three warps a scheduler is what the registers of the
-// outputs allow.  One sequence of 131072 keys, 32 heads over 8: 64 us (2.4 TB/s of
-// cache); 64 ragged sequences up to 8192 keys: 92 us; 16 sequences with five drafted
-// tokens of 64 heads over 8: 62 us; 585 keys: 9.3 us, most of it latency.
+// outputs allow.  One sequence of 131072 keys, 32 heads over 8: 65 us (2.3 TB/s of
+// cache); 64 ragged sequences up to 8192 keys: 95 us; 16 sequences with five drafted
+// tokens of 64 heads over 8: 61 us; 585 keys: 9.5 us under a page table with room for
+// as many, 12.2 under one with room for 8192, most of it latency.
 //
 // Items.  The query rows (token, head) of one sequence that share a K/V head
 // are cut into blocks of 8 * NG rows; (sequence, row block, K/V head) is an
@@ -26,7 +27,8 @@
 // Products, on the warp-level tensor cores (mma.m16n8k16, f16 in, f32 out),
 // with the codes as exact small integers and the f16 scales applied in f32:
 //   S: A = queries (f32 queries as f16 hi rows 0-7 and lo rows 8-15 of one
-//      tile, ~2^-22; 16-bit queries exactly, rows scaled by a power of two),
+//      tile, ~2^-22; 16-bit queries exactly down to 2^-27 of the row's largest; rows
+//      scaled by a power of two),
 //      B = key codes; the sum over each 32 dims is multiplied by the key's scale;
 //   O: A = value codes (16 dims x 16 keys), B = p_j * scale_j (f16 hi, and lo
 //      where the output is f32), one B for each 32 dims.

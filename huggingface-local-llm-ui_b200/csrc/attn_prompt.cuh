@@ -26,9 +26,11 @@
 // the issuing warp converged, with one elected thread, 981 -> 910 us (a branch on the
 // lane moved every descriptor between register files); the next item's geometry
 // under the last product and stores of 64 consecutive bytes, 910 -> 893 (16 ragged
-// prompts 172 -> 157).  That is a burst; where the power cap holds the clock at 1.6
-// to 1.7 GHz it takes 1050.  16 tokens behind 2048, 32 heads over 8: 23 us in halves,
-// 32.5 without (512 tokens behind 2048: 29 and 39).  Tried on the 984 us form: a
+// prompts 172 -> 157); the look at an edge tile as a sum of 0 * value, which the last
+// product of every item waits for, 512 tokens 12.9 -> 11.7, the ragged prompts 159 ->
+// 155.  That is a burst; where the power cap holds the clock at 1.6 to 1.7 GHz it takes
+// 1050 to 1090.  16 tokens behind 2048, 32 heads over 8: 22 us in halves, 32.5 without
+// (512 tokens behind 2048: 27 and 39).  Tried on the 984 us form: a
 // quarter of the exponentials by a polynomial on the FMA units, 1040; two threads to
 // a row, 1027; key tiles of 64 with two score buffers, 1270 (a score product of 64
 // keys takes as long as one of 128: its A operand's trip from shared memory).

@@ -308,8 +308,8 @@ __device__ __forceinline__ void kv_rows_of(const KvBatch& b, int row0, int rows,
 // stream of rows in and out, and close behind it the quantiser's instructions: the
 // kind of a row (query, key, value) is known to the code of its turn, and four
 // CTAs share an SM (64 registers; the rotations come from L1 again for each row).
-// 8192 bf16 tokens of 32 + 2 * 8 heads: 73 us, 43 of them the stream at the copy's
-// rate; 103 with the rotations in registers and two CTAs an SM.  The first
+// 8192 tokens of 32 + 2 * 8 heads, f32 rows in and bf16 queries out: 73 us, 43 of them
+// the stream at the copy's rate; 103 with the rotations in registers and two CTAs an SM.  The first
 // rows are on their way before it is known where they go (sequence, page: three
 // dependent loads).
 constexpr int kAppendThreads = 256;

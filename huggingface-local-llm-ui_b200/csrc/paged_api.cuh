@@ -361,15 +361,15 @@ b2q_status b2q_attn_paged_dev(b2q_engine* e, const b2q_kv_config* cfg, const b2q
   const bool split = ot == kElF32;
   // Few items that the page table keeps short: a cluster of CTAs to each, the more
   // the better down to half a block of keys a warp, and no second launch.  Device
-  // times so / by the line, 8 K/V heads: one sequence of 100 tokens 8.1 / 8.9 us, 585
-  // 9.3 / 11.8, 2048 11.5 / 13.3; four of 1024 11.7 / 13.6, of 2048 (2.7 blocks a
-  // warp) 16.1 / 14.6: the line leaves no SM without work.
+  // times so / by the line, 8 K/V heads: one sequence of 100 tokens 7.8 / 8.9 us, 585
+  // 9.5 / 12.2, 2048 11.7 / 13.4; four of 1024 11.7 / 13.8, of 2048 (2.7 blocks a
+  // warp, without this limit) 16.1 / 14.6: the line leaves no SM without work.
   // (sequences with rows: k at most, so row blocks: (rows + k (R - 1)) / R at most)
   const int warps = pg_warps(wide ? 2 : 1), R = pg_rows(wide ? 2 : 1);
   const int64_t k = std::min(a.b.n_seqs, a.b.n_tokens);
   const int64_t few = std::min(((int64_t)a.b.n_tokens * a.G + k * (R - 1)) / R, (int64_t)a.b.n_tokens * ((a.G + R - 1) / R)) * a.b.KV;
   // (the larger a cluster the fewer SMs a GPU full of them reaches: 16 of eight CTAs took
-  // two rounds, two sequences of 585 tokens 16.7 us; in clusters of four 10.5)
+  // two rounds, two sequences of 585 tokens 16.7 us; in clusters of four 10.6)
   int cluster = 1;
   if (blocks > warps)
     while (cluster < kPgMaxCluster && 2 * cluster * few <= (cluster == 1 ? ctas : cluster == 2 ? ctas * 7 / 8 : ctas * 2 / 3) &&
@@ -434,7 +434,7 @@ b2q_status b2q_attn_prompt_dev(b2q_engine* e, const b2q_prompt* p, const void* q
   if (!maps)
     return set_error(B2Q_ECUDA, "%s: cuTensorMapEncodeTiled failed", what);
   // two row tiles to an item; one, in halves, where those are no more than the SMs
-  // (16 tokens behind 2048: 23 us, 32 with room for a second row tile; with more items
+  // (16 tokens behind 2048: 22 us, 32 with room for a second row tile; with more items
   // than SMs two rounds of half the length gain nothing and load the keys twice)
   const int64_t hc = (int64_t)a.KV * a.chunks;
   a.nq = ((int64_t)(a.n_q / a.tpt) + a.n_seqs) * hc <= e->num_sms ? 1 : 2;
