@@ -5,7 +5,7 @@
 // The cache is read once, 18 * D bytes for 16 keys and values of a head, and
 // that stream is the floor.  What bounds the kernel is the instructions beside it
 // (some 530 a warp for 16 keys and 16 rows, half of them unpacking), issued on 43 to
-// 52 % of the cycles: two or three warps a scheduler is what the registers of the
+// 51 % of the cycles: two or three warps a scheduler is what the registers of the
 // outputs allow.  One sequence of 131072 keys, 32 heads over 8: 65 us (2.3 TB/s of
 // cache); 64 ragged sequences up to 8192 keys: 95 us; 16 sequences with five drafted
 // tokens of 64 heads over 8: 61 us; 585 keys: 9.5 us under a page table with room for
